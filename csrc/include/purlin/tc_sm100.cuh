@@ -178,6 +178,18 @@ PURLIN_D uint64_t smemDescSw128(uint32_t smemByteAddr) {
 PURLIN_D uint32_t instrDescBf16(uint32_t n, uint32_t m = 128u) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
+// Operand tile whose rows or columns (the index that is not summed over) are contiguous, 128-byte swizzle: blocks of 64 such indexes (128 B)
+// by 64 k rows, as a TMA box of 64 x 64 bf16 lays them down. Stride offset 1024 B between groups of 8 k rows, leading offset
+// 8192 B between blocks. A step of 16 in k is 2048 B.
+PURLIN_D uint64_t smemDescSw128MnMajor(uint32_t smemByteAddr) {
+  const uint32_t lo = ((smemByteAddr >> 4) & 0x3FFFu) | ((8192u >> 4) << 16);
+  const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+  return uint64_t(lo) | (uint64_t(hi) << 32);
+}
+constexpr uint32_t kInstrDescAMnMajor = 1u << 15, kInstrDescBMnMajor = 1u << 16;
+PURLIN_D void stShared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 
 // ---- MMA ----
 PURLIN_D void mma(uint32_t tmemD, uint64_t aDesc, uint64_t bDesc, uint32_t iDesc, uint32_t accumulate) {

@@ -46,8 +46,8 @@
 #include "purlin/layout.hpp"
 #include "purlin/tc_sm100.cuh"
 #include "purlin/telemetry.hpp"
+#include "purlin/tensor_map.hpp"
 
-namespace purlin { void setError(const std::string& e); }
 using namespace purlin;
 
 namespace {
@@ -127,9 +127,6 @@ PURLIN_D float bf16lo(uint32_t w) { return __uint_as_float(w << 16); }
 PURLIN_D float bf16hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 PURLIN_D float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 
-PURLIN_D void stShared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
 PURLIN_D Vec16 ldShared16(uint32_t addr) {
   Vec16 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x[0]), "=r"(v.x[1]), "=r"(v.x[2]), "=r"(v.x[3]) : "r"(addr) : "memory");
@@ -488,7 +485,7 @@ gemmKernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
 #pragma unroll
         for (int j = 0; j < kOut / 8; ++j) {
           const int chunk = slot * (kOut / 8) + j;
-          stShared16(rowAddr + (uint32_t(chunk ^ (lane & 7)) << 4), o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          tc::stShared16(rowAddr + (uint32_t(chunk ^ (lane & 7)) << 4), o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
         }
       };
 
@@ -628,35 +625,10 @@ gemmKernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
 // ------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encodeFn() {
-  static EncodeFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
-    return reinterpret_cast<EncodeFn>(p);
-  }();
-  return fn;
-}
-
 // [rows, cols] bf16 row-major; box = boxRows x 64 columns (128 bytes), 128-byte swizzle. Operands are loaded through
 // such maps (128 or fewer rows per box), the output is stored through one with 32-row boxes (one epilogue warp's rows).
 bool makeMap(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t cols, uint32_t boxRows) {
-  EncodeFn fn = encodeFn();
-  if (!fn) { setError("cuTensorMapEncodeTiled is not available from this driver"); return false; }
-  if (reinterpret_cast<uintptr_t>(ptr) % 16 || (cols * 2) % 16) { setError("TMA operands need 16-byte aligned base and row pitch"); return false; }
-  const cuuint64_t dims[2] = {cols, rows};
-  const cuuint64_t strides[1] = {cols * 2};
-  const cuuint32_t box[2] = {uint32_t(kBK), boxRows};
-  const cuuint32_t elem[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, elem,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) { setError("cuTensorMapEncodeTiled failed with code " + std::to_string(int(r))); return false; }
-  return true;
+  return makeTensorMap(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ptr, rows, cols * 2, cols * 2, boxRows);
 }
 
 int smCount() {
