@@ -1,0 +1,36 @@
+/* C entry points of the 4-bit microscaled format: quantisation, the way back, and products on the block-scaled tensor cores.
+ * No counterpart in the reference; see csrc/src/mx4.cu.
+ *
+ * A tensor [rows, cols] (cols a multiple of 32) is
+ *   data    rows x cols / 2 bytes, row-major: e2m1 values, the even column in a byte's low half
+ *   scales  a byte per 32 columns of a row, a power of two 2^(byte - 127), 255: the block stands for NaNs. In the order in which the tensor
+ *           cores take them: blocks of 512 bytes for 128 rows x 128 columns, [rows / 128 up][cols / 128 up][row % 32][row / 32 % 4][col / 32 % 4];
+ *           what lies past the tensor's edges is 0. */
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+enum { PURLIN_MX4_BF16 = 0, PURLIN_MX4_FP16 = 1, PURLIN_MX4_FP32 = 2 };
+
+size_t purlin_mx4_scale_bytes(int rows, int cols);
+
+/* x [rows, cols] of `dtype`, row-major, 16-byte aligned. */
+int purlin_mx4_quantize(const void* x, int dtype, void* data, void* scales, int rows, int cols, void* stream);
+/* The values that data and scales stand for, exact in bf16 or fp32 (`dtype`). */
+int purlin_mx4_dequantize(const void* data, const void* scales, void* out, int dtype, int rows, int cols, void* stream);
+
+/* C[M, N] = A[M, K] * W[N, K]^T, fp32 accumulation, bf16 output; A and W as above. epilogue: PURLIN_EPI_STORE or PURLIN_EPI_SWIGLU (W's rows
+ * alternate 16 of gate and 16 of up, N a multiple of 32, C is [M, N / 2]). N a multiple of 8. status: as in purlin_gemm_bf16. */
+int purlin_mx4_gemm(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue,
+                    uint32_t* status, void* stream);
+/* The same with activations x [M, K] of `dtype`, which are quantised into aData and aScales (workspace) first. */
+int purlin_mx4_linear(const void* x, int dtype, void* aData, void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K,
+                      int epilogue, uint32_t* status, void* stream);
+
+#ifdef __cplusplus
+}
+#endif

@@ -1,0 +1,774 @@
+// 4-bit microscaled values: quantisation, dequantisation, and products on the block-scaled tensor cores of sm_100a.
+//
+// 32 neighbouring values of a row share a power of two, 2^e with e = floor(log2(largest magnitude)) - 2 (at least -127): the largest magnitude
+// then lies in [4, 8) and becomes 4 or 6 of the element's values 0, 0.5, 1, 1.5, 2, 3, 4, 6. x 2^-e is exact in fp32, so the one rounding is to
+// the nearest of those, ties to the even code, above 6 to 6. A block that holds an infinity or a NaN stands for NaNs.
+//
+// The product multiplies both operands as they are (kind::mxf4): the tensor core takes 64 of k at a time, scales the products of every 32
+// by the two powers and adds in fp32.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <mutex>
+#include <string>
+
+#include "purlin/gemm.h"
+#include "purlin/gemm_skinny.cuh"
+#include "purlin/mx4.h"
+#include "purlin/tc_sm100.cuh"
+#include "purlin/telemetry.hpp"
+#include "purlin/tensor_map.hpp"
+
+using namespace purlin;
+
+namespace {
+
+constexpr int kBlock = 32;                      // values that share a scale
+constexpr int kScaleRows = 128, kScaleCols = 128, kScaleBytes = 512;
+
+// ------------------------------------------------------------------------------------------
+// quantisation and the way back: bound by memory
+// ------------------------------------------------------------------------------------------
+// A thread has 8 neighbouring values, four threads a block, sixteen a word of the scales; a warp 256 columns of one row per step.
+constexpr int kVec = 8, kWarpCols = 32 * kVec, kQuantThreads = 256, kUnroll = 4;
+
+PURLIN_D uint4 ldOnce(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+template <int TYPE> struct Raw { uint4 v[TYPE == PURLIN_MX4_FP32 ? 2 : 1]; };
+template <int TYPE> PURLIN_D Raw<TYPE> loadRaw(const unsigned char* p) {
+  Raw<TYPE> r;
+  r.v[0] = ldOnce(p);
+  if constexpr (TYPE == PURLIN_MX4_FP32) r.v[1] = ldOnce(p + 16);
+  return r;
+}
+template <int TYPE> PURLIN_D void toFloats(const Raw<TYPE>& r, float (&f)[kVec]) {
+  const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+  if constexpr (TYPE == PURLIN_MX4_FP32) {
+    const uint32_t u[4] = {r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[i] = __uint_as_float(w[i]); f[4 + i] = __uint_as_float(u[i]); }
+  } else if constexpr (TYPE == PURLIN_MX4_BF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = v.x; f[2 * i + 1] = v.y;
+    }
+  }
+}
+
+PURLIN_D size_t scaleOffset(int row, int col, int colBlocks) {       // of the scale of this row's block that begins at `col`
+  return (size_t(row / kScaleRows) * size_t(colBlocks) + size_t(col / kScaleCols)) * kScaleBytes + size_t(row % 32) * 16 + size_t(row / 32 % 4) * 4 + size_t(col / kBlock % 4);
+}
+
+// One step of a warp: 256 columns of a row. Rows past the last one (up to the scales' 128) write their zeros.
+template <int TYPE>
+__global__ void __launch_bounds__(kQuantThreads) quantizeKernel(const unsigned char* __restrict__ x, unsigned char* __restrict__ data, unsigned char* __restrict__ scales,
+                                                                int rows, int cols, int steps, int64_t total) {
+  tc::gridDependencyWait();
+  tc::gridLaunchDependents();
+  constexpr int kSize = TYPE == PURLIN_MX4_FP32 ? 4 : 2;
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = int64_t(blockIdx.x) * (kQuantThreads / 32) + (threadIdx.x >> 5), warps = int64_t(gridDim.x) * (kQuantThreads / 32);
+  const int colBlocks = (cols + kScaleCols - 1) / kScaleCols;
+  for (int64_t i0 = warp; i0 < total; i0 += warps * kUnroll) {
+    Raw<TYPE> raw[kUnroll];
+    int row[kUnroll], col[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = i0 + u * warps;
+      row[u] = i < total ? int(i / steps) : INT32_MAX;
+      col[u] = int(i % steps) * kWarpCols + lane * kVec;
+      raw[u].v[0] = make_uint4(0, 0, 0, 0);
+      if constexpr (TYPE == PURLIN_MX4_FP32) raw[u].v[1] = make_uint4(0, 0, 0, 0);
+      if (row[u] < rows && col[u] < cols) raw[u] = loadRaw<TYPE>(x + (size_t(row[u]) * size_t(cols) + size_t(col[u])) * kSize);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float f[kVec];
+      toFloats<TYPE>(raw[u], f);
+      uint32_t peak = 0;                                    // magnitudes as bit patterns: a NaN is above an infinity, which is above all others
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) peak = max(peak, __float_as_uint(f[e]) & 0x7fffffffu);
+      peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+      peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+      const bool finite = peak < 0x7f800000u;
+      const int scale = finite ? max(int(peak >> 23) - 2, 0) : 255;
+      const float inverse = finite ? __uint_as_float(uint32_t(254 - scale) << 23) : 0.f;
+      uint32_t codes = 0;
+#pragma unroll
+      for (int e = 0; e < kVec; e += 2) {
+        const float2 v = finite ? make_float2(f[e] * inverse, f[e + 1] * inverse) : make_float2(0.f, 0.f);
+        codes |= uint32_t(__nv_cvt_float2_to_fp4x2(v, __NV_E2M1, cudaRoundNearest)) << (4 * e);
+      }
+      // four blocks' scales meet in the first of their sixteen threads
+      uint32_t word = uint32_t(scale) << (8 * (lane / 4 % 4));
+      word |= __shfl_xor_sync(0xffffffffu, word, 4);
+      word |= __shfl_xor_sync(0xffffffffu, word, 8);
+      if (row[u] == INT32_MAX || col[u] >= colBlocks * kScaleCols) continue;
+      if (row[u] < rows && col[u] < cols) *reinterpret_cast<uint32_t*>(data + (size_t(row[u]) * size_t(cols) + size_t(col[u])) / 2) = codes;
+      if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(scales + scaleOffset(row[u], col[u], colBlocks)) = word;
+    }
+  }
+}
+
+PURLIN_D float powerOf(uint32_t scale) {      // 2^(scale - 127); 2^-127 is below the normal numbers, 255 is the NaN
+  return __uint_as_float(scale == 255u ? 0x7fffffffu : scale ? scale << 23 : 0x00400000u);
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(kQuantThreads) dequantizeKernel(const unsigned char* __restrict__ data, const unsigned char* __restrict__ scales, unsigned char* __restrict__ out,
+                                                                  int rows, int cols, int steps, int64_t total) {
+  tc::gridDependencyWait();
+  tc::gridLaunchDependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = int64_t(blockIdx.x) * (kQuantThreads / 32) + (threadIdx.x >> 5), warps = int64_t(gridDim.x) * (kQuantThreads / 32);
+  const int colBlocks = (cols + kScaleCols - 1) / kScaleCols;
+  for (int64_t i0 = warp; i0 < total; i0 += warps * kUnroll) {
+    uint32_t codes[kUnroll], scale[kUnroll];
+    int64_t at[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = i0 + u * warps;
+      const int row = int(i / steps), col = int(i % steps) * kWarpCols + lane * kVec;
+      at[u] = i < total && col < cols ? int64_t(row) * cols + col : -1;
+      if (at[u] >= 0) {
+        codes[u] = *reinterpret_cast<const uint32_t*>(data + at[u] / 2);
+        scale[u] = scales[scaleOffset(row, col, colBlocks)];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (at[u] < 0) continue;
+      const float power = powerOf(scale[u]);
+      float f[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; e += 2) {
+        const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(__nv_fp4x2_storage_t(codes[u] >> (4 * e)), __NV_E2M1);
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+        f[e] = v.x * power;
+        f[e + 1] = v.y * power;
+      }
+      if constexpr (TYPE == PURLIN_MX4_FP32) {
+        float4* to = reinterpret_cast<float4*>(out + at[u] * 4);
+        to[0] = make_float4(f[0], f[1], f[2], f[3]);
+        to[1] = make_float4(f[4], f[5], f[6], f[7]);
+      } else {
+        *reinterpret_cast<uint4*>(out + at[u] * 2) = make_uint4(skinny::pack2(f[0], f[1]), skinny::pack2(f[2], f[3]), skinny::pack2(f[4], f[5]), skinny::pack2(f[6], f[7]));
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// the tensor core's side
+// ------------------------------------------------------------------------------------------
+constexpr int kBK = 256;                        // of k in a stage: 128 bytes of a row
+constexpr int kBM = 128, kABytes = kBM * 128;
+constexpr int kScaleStage = 1024;               // scales of 128 rows in a stage: two blocks
+constexpr int kSmemLimit = 227 * 1024;
+
+// e2m1 x e2m1 -> fp32, powers of two as scales, both operands K-major; M = 128 (one CTA) or 256 (a pair). `half`: which two of a word's
+// four scales (64 of k) the instruction takes.
+PURLIN_D uint32_t instrDescMx4(uint32_t n, uint32_t m, uint32_t half) {
+  return (half << 5) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 7) << 27) | (half << 30);
+}
+template <int CTAS> PURLIN_D void mmaMx4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scaleA, uint32_t scaleB, uint32_t accumulate) {
+  if constexpr (CTAS == 2)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate) : "memory");
+}
+// 512 bytes of scales (32 rows of 16 bytes) from shared memory into four columns of all four quarters of the TMEM lanes
+template <int CTAS> PURLIN_D void scalesToTmem(uint32_t taddr, uint32_t smemByteAddr) {
+  const uint32_t lo = ((smemByteAddr >> 4) & 0x3FFFu) | (1u << 16), hi = (128u >> 4) | (1u << 14);   // groups of 8 rows, 128 bytes apart, no swizzle
+  const uint64_t desc = uint64_t(lo) | (uint64_t(hi) << 32);
+  if constexpr (CTAS == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+struct alignas(64) Maps { CUtensorMap a, b, sa, sb, c; };
+
+// ---- many rows: 256 rows of A x up to 256 rows of W per CTA pair ----
+// One accumulator of 256 columns; the scales of a stage take the columns behind it (two sets in turn). The epilogue gives the accumulator back
+// as soon as its values are in registers, activated and packed, and stores them under the next main loop.
+constexpr int kWideThreads = 32 * 10, kWideStages = 5, kMaxCols = 256;
+constexpr int kWideStage = kABytes + kMaxCols / 2 * 128 + 3 * kScaleStage;      // [A][B half][scales A][scales B: two blocks of rows]
+constexpr int kStageTileBytes = 32 * 128, kWideStaging = 8 * kStageTileBytes;
+constexpr int kBarrierBytes = 256;
+constexpr int kScaleTmem = 256, kScaleSet = 32;                                   // columns: [A k-block 0, 1: 4 each][B k-block 0, 1: 8 each]
+constexpr size_t kWideSmem = 1024 + size_t(kWideStages) * kWideStage + kWideStaging + kBarrierBytes;
+static_assert(kWideSmem <= size_t(kSmemLimit) && kWideStage % 1024 == 0, "the ring and the staging tiles fit one CTA per SM");
+
+struct WideParams {
+  int M, N, K, bn;                    // bn: columns of a tile, a multiple of 64 (of 128 where its last wave is halved), so they lie in two row blocks of W's scales
+  int tilesM, tilesN, items, fullItems;
+  int scaleBlocks;                    // 512-byte blocks of a row block: ceil(K / 128)
+  uint32_t* status;
+  uint64_t timeoutNs;
+};
+
+struct WideItem { int row0, col0, cols; };     // first row of the pair's 256, first column and number of columns
+constexpr int kBand = 8;
+PURLIN_D WideItem wideItem(const WideParams& p, int it) {
+  const int tile = it < p.fullItems ? it : p.fullItems + ((it - p.fullItems) >> 1);
+  const int perBand = kBand * p.tilesN, band = tile / perBand, within = tile - band * perBand, first = band * kBand;
+  const int rows = min(p.tilesM - first, kBand);
+  WideItem w{(first + within % rows) * 2 * kBM, within / rows * p.bn, p.bn};
+  if (it >= p.fullItems) { w.cols = p.bn / 2; w.col0 += ((it - p.fullItems) & 1) * w.cols; }
+  return w;
+}
+
+template <bool SWIGLU>
+__global__ void __launch_bounds__(kWideThreads, 1) mx4WideKernel(const __grid_constant__ Maps maps, const __grid_constant__ WideParams p) {
+  extern __shared__ unsigned char smemRaw[];
+  const uint32_t rawAddr = tc::smemAddr(smemRaw);
+  const uint32_t base = (rawAddr + 1023u) & ~1023u;
+  unsigned char* smem = smemRaw + (base - rawAddr);
+  const uint32_t stagingAll = base + uint32_t(kWideStages) * kWideStage, barBase = stagingAll + kWideStaging;
+  auto fullBar = [&](uint32_t s) { return barBase + 8u * s; };
+  auto emptyBar = [&](uint32_t s) { return barBase + 8u * (uint32_t(kWideStages) + s); };
+  const uint32_t tmemFull = barBase + 8u * (2 * kWideStages), tmemEmpty = tmemFull + 8u;
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem + size_t(kWideStages) * kWideStage + kWideStaging + 8 * (2 * kWideStages + 2));
+  volatile uint32_t* tmemBaseWord = words;
+  volatile int* abortWord = reinterpret_cast<volatile int*>(words + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t ctaRank = tc::clusterCtaRank();
+  const int pairIdx = int(blockIdx.x) / 2, numPairs = int(gridDim.x) / 2;
+
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < kWideStages; ++s) { tc::mbarInit(fullBar(s), 1); tc::mbarInit(emptyBar(s), 1); }
+    tc::mbarInit(tmemFull, 1);
+    tc::mbarInit(tmemEmpty, 16);                       // the epilogue warps of both CTAs
+    *abortWord = 0;
+    tc::mbarFenceInit();
+    tc::tmaPrefetchDescriptor(&maps.a);
+    tc::tmaPrefetchDescriptor(&maps.b);
+  }
+  if (warp == 1) { tc::tmemAllocPair(tc::smemAddr(words), 512); tc::tmemRelinquishPair(); }
+  tc::fenceBeforeThreadSync();
+  tc::clusterSync();
+  tc::fenceAfterThreadSync();
+  tc::gridDependencyWait();
+  tc::gridLaunchDependents();
+  const uint32_t tmemBase = *tmemBaseWord;
+  const uint32_t leaderBars = tc::mapToCta(barBase, 0);
+  const int kBlocks = (p.K + kBK - 1) / kBK;
+  const int lastBlockA = (p.M - 1) / kScaleRows, lastBlockW = (p.N - 1) / kScaleRows;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t st = 0, ph = 0;
+      bool ok = true;
+      for (int it = pairIdx; it < p.items && ok; it += numPairs) {
+        const WideItem w = wideItem(p, it);
+        const int half = w.cols / 2, loads = w.cols == p.bn ? 2 : 1, box = p.bn / 4;
+        const int aRow = w.row0 + int(ctaRank) * kBM, bRow = w.col0 + int(ctaRank) * half;
+        // Row blocks of the scales: this CTA's rows of A, all columns of the tile. Blocks past the last one (their values are zeros and their
+        // results are not stored) take the last one's.
+        const int sa = min(aRow / kScaleRows, lastBlockA), sb = w.col0 / kScaleRows, sbs = (w.col0 + w.cols - 1) / kScaleRows - sb + 1;
+        const uint32_t bytes = uint32_t(2 * (kABytes + half * 128 + (1 + sbs) * kScaleStage));
+        for (int kb = 0; kb < kBlocks; ++kb) {
+          ok = tc::mbarWait(emptyBar(st), ph ^ 1, abortWord, p.timeoutNs);
+          if (!ok) { skinny::recordTimeout(p.status, 1, it, kb); break; }
+          const uint32_t sA = base + st * kWideStage, sB = sA + kABytes, sS = sB + kMaxCols / 2 * 128;
+          const uint32_t full = leaderBars + 8u * st;
+          if (ctaRank == 0) tc::mbarExpectTx(fullBar(st), bytes);
+          tc::tmaLoad2dPair(sA, &maps.a, kb * 128, aRow, full);
+          for (int i = 0; i < loads; ++i) tc::tmaLoad2dPair(sB + uint32_t(i * box * 128), &maps.b, kb * 128, bRow + i * box, full);
+          tc::tmaLoad2dPair(sS, &maps.sa, 0, (sa * p.scaleBlocks + 2 * kb) * 4, full);
+          for (int i = 0; i < sbs; ++i) tc::tmaLoad2dPair(sS + uint32_t((1 + i) * kScaleStage), &maps.sb, 0, (min(sb + i, lastBlockW) * p.scaleBlocks + 2 * kb) * 4, full);
+          if (++st == kWideStages) { st = 0; ph ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && ctaRank == 0) {
+      uint32_t st = 0, ph = 0, use = 0, set = 0;
+      bool ok = true;
+      const uint64_t descA0 = tc::smemDescSw128(base), descB0 = tc::smemDescSw128(base + kABytes);
+      for (int it = pairIdx; it < p.items && ok; it += numPairs, ++use) {
+        const WideItem w = wideItem(p, it);
+        const uint32_t sbs = uint32_t((w.col0 + w.cols - 1) / kScaleRows - w.col0 / kScaleRows + 1), shift = uint32_t(w.col0 % kScaleRows / 32);
+        const uint32_t idesc = instrDescMx4(uint32_t(w.cols), 2 * kBM, 0), idescHigh = instrDescMx4(uint32_t(w.cols), 2 * kBM, 1);
+        ok = tc::mbarWait(tmemEmpty, (use & 1) ^ 1, abortWord, p.timeoutNs);
+        if (!ok) { skinny::recordTimeout(p.status, 2, it, 0); break; }
+        for (int kb = 0; kb < kBlocks; ++kb, set ^= 1) {
+          ok = tc::mbarWait(fullBar(st), ph, abortWord, p.timeoutNs);
+          if (!ok) { skinny::recordTimeout(p.status, 3, it, kb); break; }
+          tc::fenceAfterThreadSync();
+          // 64 of k to an MMA, 128 to a block of scales; what lies past K is neither scaled nor multiplied
+          const int left = p.K - kb * kBK, steps = min((left + 63) / 64, 4), blocks = min((left + 127) / 128, 2);
+          const uint32_t sS = base + st * kWideStage + kABytes + kMaxCols / 2 * 128;
+          const uint32_t scaleA = tmemBase + kScaleTmem + set * kScaleSet, scaleB = scaleA + 8;
+          for (int q = 0; q < blocks; ++q) {
+            scalesToTmem<2>(scaleA + 4u * q, sS + uint32_t(q * kScaleBytes));
+            for (uint32_t i = 0; i < sbs; ++i) scalesToTmem<2>(scaleB + 8u * q + 4u * i, sS + (1 + i) * kScaleStage + uint32_t(q * kScaleBytes));
+          }
+          const uint64_t da = descA0 + uint64_t(st * (kWideStage >> 4)), db = descB0 + uint64_t(st * (kWideStage >> 4));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < steps)
+              mmaMx4<2>(tmemBase, da + 2 * k, db + 2 * k, k & 1 ? idescHigh : idesc, scaleA + 4u * (k / 2), scaleB + 8u * (k / 2) + shift, uint32_t((kb | k) != 0));
+          tc::mmaCommitPairs(emptyBar(st), 3u);
+          if (++st == kWideStages) { st = 0; ph ^= 1; }
+        }
+        if (ok) tc::mmaCommitPairs(tmemFull, 3u);
+      }
+    }
+  } else {
+    // ---- epilogue: two warps per quarter of the lanes, each up to two units of 64 accumulator columns ----
+    constexpr int kOutWords = SWIGLU ? 16 : 32;        // packed outputs of a unit
+    const int quarter = warp & 3, half = (warp - 2) / 4;
+    const uint32_t buf = stagingAll + uint32_t(warp - 2) * kStageTileBytes;
+    uint32_t use = 0;
+    bool ok = true;
+    for (int it = pairIdx; it < p.items && ok; it += numPairs, ++use) {
+      const WideItem w = wideItem(p, it);
+      const int units = w.cols / 64, first = half ? (units + 1) / 2 : 0, count = half ? units / 2 : (units + 1) / 2;
+      const int row0 = w.row0 + int(ctaRank) * kBM + quarter * 32;
+      ok = tc::mbarWait(tmemFull, use & 1, abortWord, p.timeoutNs);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) { if (lane == 0) skinny::recordTimeout(p.status, 5, it, 0); break; }
+      tc::fenceAfterThreadSync();
+      const uint32_t taddr = tmemBase + (uint32_t(quarter * 32) << 16) + uint32_t(first * 64);
+      uint32_t o[2][kOutWords];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (u < count) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t r[32];
+            tc::tmemLoad32(taddr + uint32_t(u * 64 + c * 32), r);
+            tc::tmemLoadWaitFor(r);
+            if constexpr (SWIGLU) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                o[u][c * 8 + i] = skinny::pack2(skinny::siluOf(__uint_as_float(r[2 * i])) * __uint_as_float(r[16 + 2 * i]),
+                                                skinny::siluOf(__uint_as_float(r[2 * i + 1])) * __uint_as_float(r[17 + 2 * i]));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[u][c * 16 + i] = skinny::pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+            }
+          }
+        }
+      }
+      tc::fenceBeforeThreadSync();
+      __syncwarp();
+      if (lane == 0) tc::mbarArriveClusterTmem(leaderBars + 8u * (2 * kWideStages + 1));
+      // staging: 32 rows of 128 bytes (64 columns), or of 64 bytes (32 columns) with the gate, swizzled as the store's map says
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (u < count) {
+          if (lane == 0) tc::bulkWaitGroupRead<0>();
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < kOutWords / 4; ++j) {
+            const uint32_t at = SWIGLU ? uint32_t(lane) * 64u + (uint32_t(j) ^ uint32_t(lane >> 1 & 3)) * 16u : uint32_t(lane) * 128u + (uint32_t(j) ^ uint32_t(lane & 7)) * 16u;
+            tc::stShared16(buf + at, o[u][4 * j], o[u][4 * j + 1], o[u][4 * j + 2], o[u][4 * j + 3]);
+          }
+          tc::fenceProxyAsyncShared();
+          __syncwarp();
+          const int acc = w.col0 + (first + u) * 64;
+          if (lane == 0) { tc::tmaStore2d(&maps.c, SWIGLU ? acc / 2 : acc, row0, buf); tc::bulkCommitGroup(); }
+        }
+      }
+    }
+    if (lane == 0) tc::bulkWaitGroup<0>();
+  }
+
+  if (*abortWord) tc::landingPause();
+  tc::fenceBeforeThreadSync();
+  tc::clusterSync();
+  if (warp == 1) tc::tmemDeallocPair(tmemBase, 512);
+}
+
+// ---- few rows: 128 rows of W are the rows of the MMA, the activations its columns, k split over a cluster ----
+// As in gemm_skinny.cuh: what bounds it is the read of W, every byte of which passes one SM once; the fp32 partial tiles are added in distributed
+// shared memory in ascending k order.
+constexpr int kFewThreads = skinny::kThreads, kFewTokens = 128, kWRows = 128;
+
+struct FewParams {
+  int N, K, tokens, cols;              // cols: columns of the MMA, tokens rounded up to 16
+  int stages, tmemCols, ahead;
+  int scaleBlocks;
+  __nv_bfloat16* C;
+  int ldc;
+  uint32_t* status;
+  uint64_t timeoutNs;
+};
+PURLIN_HD int fewStageBytes(int cols) { return kABytes + cols * 128 + 2 * kScaleStage; }     // [W][X][scales W][scales X]
+
+template <bool SWIGLU>
+__global__ void __launch_bounds__(kFewThreads, 2) mx4FewKernel(const __grid_constant__ Maps maps, const __grid_constant__ FewParams p) {
+  extern __shared__ unsigned char smemRaw[];
+  const uint32_t rawAddr = tc::smemAddr(smemRaw);
+  const uint32_t base = (rawAddr + 1023u) & ~1023u;
+  unsigned char* smem = smemRaw + (base - rawAddr);
+  const uint32_t stageBytes = uint32_t(fewStageBytes(p.cols));
+  const uint32_t barBase = base + uint32_t(p.stages) * stageBytes;
+  auto fullBar = [&](uint32_t s) { return barBase + 8u * s; };
+  auto emptyBar = [&](uint32_t s) { return barBase + 8u * (uint32_t(p.stages) + s); };
+  const uint32_t accFull = barBase + 8u * (2u * uint32_t(p.stages)), mmasDone = accFull + 8u;
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem + size_t(p.stages) * stageBytes + 8 * (2 * p.stages + 2));
+  volatile uint32_t* tmemBaseWord = words;
+  volatile int* abortWord = reinterpret_cast<volatile int*>(words + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t split;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(split));
+  const uint32_t part = tc::clusterCtaRank();
+  const int tile = int(blockIdx.x / split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) { tc::mbarInit(fullBar(s), 1); tc::mbarInit(emptyBar(s), 1); }
+    tc::mbarInit(accFull, 1);
+    tc::mbarInit(mmasDone, 1);
+    *abortWord = 0;
+    tc::mbarFenceInit();
+    tc::tmaPrefetchDescriptor(&maps.a);
+    tc::tmaPrefetchDescriptor(&maps.b);
+  }
+  const int kBlocks = (p.K + kBK - 1) / kBK;
+  const int kBegin = int(int64_t(kBlocks) * part / split), kEnd = int(int64_t(kBlocks) * (part + 1) / split);
+  // The first lap of the ring is asked into L2 while the kernel before this one (the quantisation of the activations) drains.
+  if (warp == 0 && lane == 0)
+    for (int kb = kBegin; kb < min(kEnd, kBegin + p.ahead); ++kb) tc::tmaPrefetchL2(&maps.a, kb * 128, tile * kWRows);
+  if (warp == 1) { tc::tmemAlloc(tc::smemAddr(words), uint32_t(p.tmemCols)); tc::tmemRelinquish(); }
+  tc::gridDependencyWait();
+  tc::fenceBeforeThreadSync();
+  __syncthreads();
+  tc::fenceAfterThreadSync();
+  const uint32_t tmemBase = *tmemBaseWord;
+  uint32_t peer[skinny::kMaxSplit];
+#pragma unroll
+  for (int q = 0; q < skinny::kMaxSplit; ++q) peer[q] = uint32_t(q) < split ? tc::mapToCta(base, uint32_t(q)) : 0u;
+
+  bool ok = true;
+  uint32_t st = 0, ph = 0;
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t bytes = stageBytes;
+      for (int kb = kBegin; kb < kEnd && ok; ++kb) {
+        ok = tc::mbarWait(emptyBar(st), ph ^ 1, abortWord, p.timeoutNs);
+        if (!ok) { skinny::recordTimeout(p.status, 1, tile, kb); break; }
+        const uint32_t sW = base + st * stageBytes, sX = sW + kABytes, sS = sX + uint32_t(p.cols * 128);
+        tc::mbarExpectTx(fullBar(st), bytes);
+        tc::tmaLoad2d(sW, &maps.a, kb * 128, tile * kWRows, fullBar(st));
+        tc::tmaLoad2d(sS, &maps.sa, 0, (tile * p.scaleBlocks + 2 * kb) * 4, fullBar(st));
+        tc::tmaLoad2d(sX, &maps.b, kb * 128, 0, fullBar(st));
+        tc::tmaLoad2d(sS + kScaleStage, &maps.sb, 0, 2 * kb * 4, fullBar(st));
+        if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = instrDescMx4(uint32_t(p.cols), kWRows, 0), idescHigh = instrDescMx4(uint32_t(p.cols), kWRows, 1);
+      const uint64_t descW = tc::smemDescSw128(base), descX = tc::smemDescSw128(base + kABytes);
+      const uint32_t scales = tmemBase + uint32_t((p.cols + 31) / 32 * 32);
+      uint32_t set = 0;
+      for (int kb = kBegin; kb < kEnd && ok; ++kb, set ^= 1) {
+        ok = tc::mbarWait(fullBar(st), ph, abortWord, p.timeoutNs);
+        if (!ok) { skinny::recordTimeout(p.status, 3, tile, kb); break; }
+        tc::fenceAfterThreadSync();
+        const int left = p.K - kb * kBK, steps = min((left + 63) / 64, 4), blocks = min((left + 127) / 128, 2);
+        const uint32_t sS = base + st * stageBytes + kABytes + uint32_t(p.cols * 128);
+        const uint32_t scaleW = scales + set * 16, scaleX = scaleW + 8;
+        for (int q = 0; q < blocks; ++q) {
+          scalesToTmem<1>(scaleW + 4u * q, sS + uint32_t(q * kScaleBytes));
+          scalesToTmem<1>(scaleX + 4u * q, sS + kScaleStage + uint32_t(q * kScaleBytes));
+        }
+        const uint64_t step = uint64_t(st * (stageBytes >> 4));
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < steps)
+            mmaMx4<1>(tmemBase, descW + step + 2 * k, descX + step + 2 * k, k & 1 ? idescHigh : idesc, scaleW + 4u * (k / 2), scaleX + 4u * (k / 2), uint32_t(kb != kBegin || k != 0));
+        tc::mmaCommit(emptyBar(st));
+        if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
+      }
+      if (ok) tc::mmaCommit(accFull);
+    }
+  } else {
+    // ---- this CTA's partial tile: TMEM (lane = row of W, column = token) -> shared memory [token][row of W] ----
+    const int quarter = warp & 3;
+    ok = tc::mbarWait(accFull, 0, abortWord, p.timeoutNs);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok && lane == 0) skinny::recordTimeout(p.status, 5, tile, 0);
+    if (ok) {
+      // every load has landed and every MMA has read its stage, so the stages' memory is free
+      tc::fenceAfterThreadSync();
+      const uint32_t taddr = tmemBase + (uint32_t(quarter * 32) << 16);
+      float* mine = reinterpret_cast<float*>(smem) + quarter * 32 + lane;
+      for (int c = 0; c < p.tokens; c += 32) {
+        uint32_t r[32];
+        tc::tmemLoad32(taddr + uint32_t(c), r);
+        tc::tmemLoadWaitFor(r);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) if (c + i < p.tokens) mine[size_t(c + i) * kWRows] = __uint_as_float(r[i]);
+      }
+      tc::fenceBeforeThreadSync();
+    }
+  }
+  if (!ok) {                            // the partial tile of this CTA is not what its peers would add: they learn of it through their abort words
+    const uint32_t word = tc::smemAddr(words + 1);
+    for (uint32_t q = 0; q < split; ++q) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::mapToCta(word, q)), "r"(1) : "memory");
+  }
+  __syncwarp();
+  tc::clusterSync();                    // every partial tile of the cluster is in shared memory
+  tc::gridLaunchDependents();
+  if (*abortWord == 0) {
+    constexpr int kOut = SWIGLU ? kWRows / 2 : kWRows, kPieces = kOut / 8;
+    const int outCols = SWIGLU ? p.N / 2 : p.N, n0 = tile * kOut;
+    const int begin = int(int64_t(p.tokens) * kPieces * part / split), end = int(int64_t(p.tokens) * kPieces * (part + 1) / split);
+    for (int i = begin + int(threadIdx.x); i < end; i += kFewThreads) {
+      const int t = i / kPieces, piece = i % kPieces;
+      if (n0 + piece * 8 + 8 > outCols) continue;
+      float v[8];
+      if constexpr (SWIGLU) {
+        const uint32_t at = uint32_t(t * kWRows + (piece >> 1) * 32 + (piece & 1) * 8) * 4u;
+        float u[8];
+        skinny::sumPartials(peer, int(split), at, v);
+        skinny::sumPartials(peer, int(split), at + 64u, u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = skinny::siluOf(v[e]) * u[e];
+      } else {
+        skinny::sumPartials(peer, int(split), uint32_t(t * kWRows + piece * 8) * 4u, v);
+      }
+      st16(p.C + size_t(t) * p.ldc + n0 + piece * 8, Vec16{{skinny::pack2(v[0], v[1]), skinny::pack2(v[2], v[3]), skinny::pack2(v[4], v[5]), skinny::pack2(v[6], v[7])}});
+    }
+  }
+  tc::clusterSync();                    // nobody leaves behind a partial tile that a peer still reads
+  if (*abortWord) {
+    if (warp == 0 && lane == 0) for (uint32_t s = 0; s < uint32_t(p.stages); ++s) tc::mbarDrain(fullBar(s), s < st ? ph : ph ^ 1);
+    if (warp == 1 && lane == 0) { tc::mmaCommit(mmasDone); tc::mbarDrain(mmasDone, 0); }
+    __syncwarp();
+  }
+  tc::fenceBeforeThreadSync();
+  __syncthreads();
+  if (warp == 1) tc::tmemDealloc(tmemBase, uint32_t(p.tmemCols));
+}
+
+// ------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------
+struct Device { int sms = 0, index = -1; };
+bool currentDevice(Device& d) {
+  static std::mutex mu;
+  static int sms[64] = {};
+  if (cudaGetDevice(&d.index) != cudaSuccess || d.index < 0 || d.index >= 64) { setError("mx4 launch: no current device"); return false; }
+  std::lock_guard<std::mutex> lock(mu);
+  if (!sms[d.index]) cudaDeviceGetAttribute(&sms[d.index], cudaDevAttrMultiProcessorCount, d.index);
+  d.sms = sms[d.index];
+  return d.sms > 0;
+}
+
+bool launched(cudaError_t e) {
+  if (e != cudaSuccess) setError(std::string("mx4 launch: ") + cudaGetErrorString(e));
+  return e == cudaSuccess;
+}
+
+bool sizesFit(int rows, int cols) {
+  if (rows <= 0 || cols <= 0) { setError("mx4: dimensions must be positive"); return false; }
+  if (cols % kBlock) { setError("mx4: the columns must be a multiple of 32"); return false; }
+  if (rows > INT32_MAX - kScaleRows || cols > INT32_MAX - kWarpCols) { setError("mx4: dimensions too large"); return false; }
+  return true;
+}
+
+template <typename... A>
+int launchRows(void (*kernel)(A...), int64_t total, const Device& dev, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
+  constexpr int kWarps = kQuantThreads / 32;
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>((total + kWarps - 1) / kWarps, int64_t(dev.sms) * 8)));
+  cfg.blockDim = dim3(kQuantThreads); cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 1;
+  return launched(cudaLaunchKernelEx(&cfg, kernel, args...)) ? 0 : 1;
+}
+
+// rows of 128 bytes without a swizzle, eight of them (the scales of 128 rows x 256 columns) to a box
+bool scaleMap(CUtensorMap* map, const void* ptr, uint64_t bytes) {
+  const TensorMapEncodeFn fn = tensorMapEncodeFn();
+  if (!fn) { setError("cuTensorMapEncodeTiled is not available from this driver"); return false; }
+  if (reinterpret_cast<uintptr_t>(ptr) % 16) { setError("TMA operands need 16-byte aligned base and row pitch"); return false; }
+  const cuuint64_t dims[2] = {128, bytes / 128}, strides[1] = {128};
+  const cuuint32_t box[2] = {128, kScaleStage / 128}, elem[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { setError("cuTensorMapEncodeTiled failed with code " + std::to_string(int(r))); return false; }
+  return true;
+}
+// the output, in boxes of 32 rows x 64 bytes (32 columns)
+bool narrowOutputMap(CUtensorMap* map, void* ptr, uint64_t rows, uint64_t cols) {
+  const TensorMapEncodeFn fn = tensorMapEncodeFn();
+  if (reinterpret_cast<uintptr_t>(ptr) % 16 || cols * 2 % 16) { setError("TMA operands need 16-byte aligned base and row pitch"); return false; }
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols * 2};
+  const cuuint32_t box[2] = {32, 32}, elem[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { setError("cuTensorMapEncodeTiled failed with code " + std::to_string(int(r))); return false; }
+  return true;
+}
+
+size_t scaleBytes(int rows, int cols) { return size_t((rows + kScaleRows - 1) / kScaleRows) * size_t((cols + kScaleCols - 1) / kScaleCols) * kScaleBytes; }
+
+bool optIn(const void* kernel, bool& done) {
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  if (!done && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit) != cudaSuccess) { setError("cannot opt in to 227 KiB of shared memory"); return false; }
+  done = true;
+  return true;
+}
+
+int launchFew(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, bool swiglu, uint32_t* status, const Device& dev,
+              cudaStream_t stream) {
+  const int outCols = swiglu ? N / 2 : N;
+  if (reinterpret_cast<uintptr_t>(C) % 16) { setError("TMA operands need 16-byte aligned base and row pitch"); return 1; }
+  FewParams p{};
+  p.N = N; p.K = K; p.tokens = M; p.cols = (M + 15) / 16 * 16; p.scaleBlocks = (K + kScaleCols - 1) / kScaleCols;
+  p.C = static_cast<__nv_bfloat16*>(C); p.ldc = outCols; p.status = status; p.timeoutNs = 2ull * 1000 * 1000 * 1000;
+  const int tiles = (N + kWRows - 1) / kWRows, kBlocks = (K + kBK - 1) / kBK;
+  // k is cut while that brings more CTAs to work (two to an SM) and leaves each at least four k-blocks
+  int split = 1;
+  while (split < skinny::kMaxSplit && int64_t(tiles) * split * 2 <= 2 * int64_t(dev.sms) && kBlocks >= 8 * split) split *= 2;
+  const int used = (p.cols + 31) / 32 * 32 + 32;
+  p.tmemCols = used <= 64 ? 64 : used <= 128 ? 128 : 256;
+  // the partial tile [tokens][128] in fp32 takes the place of the stages
+  const int room = 113 * 1024 - 1024 - 256, stage = fewStageBytes(p.cols);
+  p.stages = std::max(std::min({room / stage, 8, std::max((kBlocks + split - 1) / split, 2)}), (M * kWRows * 4 + stage - 1) / stage);
+  p.ahead = std::min(p.stages, 4);
+  Maps maps{};
+  if (!makeTensorMap(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, wData, uint64_t(N), uint64_t(K) / 2, uint64_t(K) / 2, kWRows) ||
+      !makeTensorMap(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, aData, uint64_t(M), uint64_t(K) / 2, uint64_t(K) / 2, uint32_t(p.cols)) ||
+      !scaleMap(&maps.sa, wScales, scaleBytes(N, K)) || !scaleMap(&maps.sb, aScales, scaleBytes(M, K))) return 1;
+  auto kernel = swiglu ? mx4FewKernel<true> : mx4FewKernel<false>;
+  static bool done[64][2] = {};
+  if (!optIn(reinterpret_cast<const void*>(kernel), done[dev.index][swiglu])) return 1;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = unsigned(split); attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(unsigned(tiles) * unsigned(split)); cfg.blockDim = dim3(kFewThreads); cfg.stream = stream;
+  cfg.dynamicSmemBytes = size_t(p.stages) * size_t(stage) + 256 + 1024; cfg.attrs = attr; cfg.numAttrs = 2;
+  return launched(cudaLaunchKernelEx(&cfg, kernel, maps, p)) ? 0 : 1;
+}
+
+int launchWide(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, bool swiglu, uint32_t* status, const Device& dev,
+               cudaStream_t stream) {
+  auto kernel = swiglu ? mx4WideKernel<true> : mx4WideKernel<false>;
+  static bool done[64][2] = {};
+  if (!optIn(reinterpret_cast<const void*>(kernel), done[dev.index][swiglu])) return 1;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.blockDim = dim3(kWideThreads); cfg.stream = stream; cfg.dynamicSmemBytes = kWideSmem; cfg.attrs = attr;
+  static std::mutex mu;
+  static int known[64][2] = {};
+  int pairs;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    int& n = known[dev.index][swiglu];
+    if (!n) {                           // pairs must sit on SMs of one GPC: ask how many the device can hold at once
+      n = dev.sms / 2;
+      cfg.gridDim = dim3(unsigned(dev.sms / 2 * 2)); cfg.numAttrs = 1;
+      int m = 0;
+      if (cudaOccupancyMaxActiveClusters(&m, kernel, &cfg) == cudaSuccess && m > 0) n = std::min(n, m);
+    }
+    pairs = n;
+  }
+  WideParams p{};
+  p.M = M; p.N = N; p.K = K; p.scaleBlocks = (K + kScaleCols - 1) / kScaleCols; p.status = status; p.timeoutNs = 2ull * 1000 * 1000 * 1000;
+  p.tilesM = (M + 2 * kBM - 1) / (2 * kBM);
+  // the width that is expected to take least: a tile costs its columns and about 48 columns' worth besides (fill, drain, the loads of A)
+  double least = 1e30;
+  for (int bn : {256, 192, 128}) {
+    const int tilesN = (N + bn - 1) / bn, tiles = p.tilesM * tilesN, rest = tiles % pairs;
+    const bool halved = bn % 128 == 0 && tiles > pairs && rest > 0 && 2 * rest <= pairs;
+    const double cost = double(tiles / pairs) * (bn + 48) + (rest ? (halved ? bn / 2 : bn) + 48 : 0);
+    if (cost < least) {
+      least = cost;
+      p.bn = bn; p.tilesN = tilesN;
+      p.fullItems = halved ? tiles - rest : tiles;
+      p.items = halved ? p.fullItems + 2 * rest : tiles;
+    }
+  }
+  const int outCols = swiglu ? N / 2 : N;
+  Maps maps{};
+  if (!makeTensorMap(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, aData, uint64_t(M), uint64_t(K) / 2, uint64_t(K) / 2, kBM) ||
+      !makeTensorMap(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, wData, uint64_t(N), uint64_t(K) / 2, uint64_t(K) / 2, uint32_t(p.bn / 4)) ||
+      !scaleMap(&maps.sa, aScales, scaleBytes(M, K)) || !scaleMap(&maps.sb, wScales, scaleBytes(N, K)) ||
+      !(swiglu ? narrowOutputMap(&maps.c, C, uint64_t(M), uint64_t(outCols))
+               : makeTensorMap(&maps.c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, C, uint64_t(M), uint64_t(outCols) * 2, uint64_t(outCols) * 2, 32))) return 1;
+  cfg.gridDim = dim3(unsigned(2 * std::min(pairs, p.items))); cfg.numAttrs = 2;
+  return launched(cudaLaunchKernelEx(&cfg, kernel, maps, p)) ? 0 : 1;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t purlin_mx4_scale_bytes(int rows, int cols) { return rows > 0 && cols > 0 ? scaleBytes(rows, cols) : 0; }
+
+int purlin_mx4_quantize(const void* x, int dtype, void* data, void* scales, int rows, int cols, void* stream) {
+  NvtxRange range("mx4Quantize", size_t(rows) * size_t(cols) / 2);
+  if (!sizesFit(rows, cols)) return 1;
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales)) % 16) { setError("mx4: tensors must start on a 16-byte boundary"); return 1; }
+  Device dev;
+  if (!currentDevice(dev)) return 1;
+  const int steps = (cols + kWarpCols - 1) / kWarpCols;
+  const int64_t total = int64_t((rows + kScaleRows - 1) / kScaleRows * kScaleRows) * steps;
+  auto kernel = dtype == PURLIN_MX4_BF16 ? quantizeKernel<PURLIN_MX4_BF16> : dtype == PURLIN_MX4_FP16 ? quantizeKernel<PURLIN_MX4_FP16>
+              : dtype == PURLIN_MX4_FP32 ? quantizeKernel<PURLIN_MX4_FP32> : nullptr;
+  if (!kernel) { setError("mx4: unknown type"); return 1; }
+  return launchRows(kernel, total, dev, static_cast<cudaStream_t>(stream), static_cast<const unsigned char*>(x), static_cast<unsigned char*>(data),
+                    static_cast<unsigned char*>(scales), rows, cols, steps, total);
+}
+
+int purlin_mx4_dequantize(const void* data, const void* scales, void* out, int dtype, int rows, int cols, void* stream) {
+  NvtxRange range("mx4Dequantize", size_t(rows) * size_t(cols) / 2);
+  if (!sizesFit(rows, cols)) return 1;
+  if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales)) % 16) { setError("mx4: tensors must start on a 16-byte boundary"); return 1; }
+  Device dev;
+  if (!currentDevice(dev)) return 1;
+  const int steps = (cols + kWarpCols - 1) / kWarpCols;
+  const int64_t total = int64_t(rows) * steps;
+  auto kernel = dtype == PURLIN_MX4_BF16 ? dequantizeKernel<PURLIN_MX4_BF16> : dtype == PURLIN_MX4_FP32 ? dequantizeKernel<PURLIN_MX4_FP32> : nullptr;
+  if (!kernel) { setError("mx4: values come back in bf16 or fp32"); return 1; }
+  return launchRows(kernel, total, dev, static_cast<cudaStream_t>(stream), static_cast<const unsigned char*>(data), static_cast<const unsigned char*>(scales),
+                    static_cast<unsigned char*>(out), rows, cols, steps, total);
+}
+
+int purlin_mx4_gemm(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue, uint32_t* status, void* stream) {
+  const bool swiglu = epilogue == PURLIN_EPI_SWIGLU;
+  NvtxRange range(swiglu ? "mx4GemmSwiglu" : "mx4Gemm", size_t(M) * size_t(N) * 2);
+  if (!sizesFit(M, K) || !sizesFit(N, K)) return 1;
+  if (epilogue != PURLIN_EPI_STORE && !swiglu) { setError("unknown epilogue"); return 1; }
+  if (N % (swiglu ? 32 : 8)) { setError(swiglu ? "the SwiGLU epilogue needs N to be a multiple of 32" : "mx4: N must be a multiple of 8"); return 1; }
+  if (int64_t(M) * N / 4096 > INT32_MAX / 4 || scaleBytes(std::max(M, N), K) / 128 > size_t(INT32_MAX)) { setError("mx4: the product is too large"); return 1; }   // tile numbers, TMA coordinates
+  Device dev;
+  if (!currentDevice(dev)) return 1;
+  return M <= kFewTokens ? launchFew(aData, aScales, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream))
+                         : launchWide(aData, aScales, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream));
+}
+
+int purlin_mx4_linear(const void* x, int dtype, void* aData, void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue, uint32_t* status, void* stream) {
+  const int rc = purlin_mx4_quantize(x, dtype, aData, aScales, M, K, stream);
+  return rc ? rc : purlin_mx4_gemm(aData, aScales, wData, wScales, C, M, N, K, epilogue, status, stream);
+}
+
+}  // extern "C"

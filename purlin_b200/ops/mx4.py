@@ -1,0 +1,171 @@
+"""4-bit microscaled tensors and products of them (csrc/src/mx4.cu).
+
+32 neighbouring values of a row share a power of two (a byte, e8m0); each is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it, with a sign (e2m1): 4.25
+bits a value. ``quantize_mx4`` makes such a tensor, ``mx4_gemm`` and ``mx4_gemm_swiglu`` multiply activations with a weight that was quantised once;
+both operands go to the block-scaled tensor cores as they are, sums are fp32. For inference: nothing here is differentiable.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from contextlib import nullcontext
+from dataclasses import dataclass
+from typing import Optional, Tuple, Union
+
+import torch
+
+from .. import _native, _stream
+
+EPI_STORE, EPI_SWIGLU = 0, 1
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_declared = False
+
+
+def _lib():
+    global _declared
+    lib = _native.cuda()
+    if not _declared:
+        vp, i = C.c_void_p, C.c_int
+        lib.purlin_mx4_scale_bytes.argtypes = [i, i]
+        lib.purlin_mx4_scale_bytes.restype = C.c_size_t
+        lib.purlin_mx4_quantize.argtypes = [vp, i, vp, vp, i, i, vp]
+        lib.purlin_mx4_dequantize.argtypes = [vp, vp, vp, i, i, i, vp]
+        lib.purlin_mx4_gemm.argtypes = [vp] * 5 + [i] * 4 + [vp, vp]
+        lib.purlin_mx4_linear.argtypes = [vp, i] + [vp] * 5 + [i] * 4 + [vp, vp]
+        _declared = True
+    return lib
+
+
+def _on(device: torch.device):
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def scale_bytes(rows: int, cols: int) -> int:
+    """Bytes of the scales of a [rows, cols] tensor: 512 for every 128 rows x 128 columns, the last ones filled up."""
+    return -(-rows // 128) * -(-cols // 128) * 512
+
+
+@dataclass(frozen=True)
+class Mx4Tensor:
+    """A [rows, cols] tensor in 4-bit microscaled form. ``data``: uint8 [rows, cols / 2], the even column in a byte's low half. ``scales``: uint8, a
+    byte b per 32 columns of a row for 2^(b - 127) (255: the block stands for NaNs), in the tensor cores' order: blocks of 512 bytes for
+    128 rows x 128 columns, [rows / 128][cols / 128][row % 32][row / 32 % 4][col / 32 % 4], zeros past the edges."""
+    data: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self):
+        d, s = self.data, self.scales
+        if d.dtype != torch.uint8 or s.dtype != torch.uint8:
+            raise TypeError("data and scales are uint8 tensors")
+        if d.dim() != 2 or d.shape[1] == 0 or d.shape[1] % 16 or s.numel() != scale_bytes(d.shape[0], 2 * d.shape[1]):
+            raise ValueError("data is [rows, cols / 2] with cols a multiple of 32, and scales has 512 bytes for every 128 rows x 128 columns")
+        if not (d.is_cuda and s.device == d.device and d.is_contiguous() and s.is_contiguous()):
+            raise ValueError("data and scales must be contiguous CUDA tensors on one device")
+        if (d.data_ptr() | s.data_ptr()) % 16:
+            raise ValueError("data and scales must start on a 16-byte boundary")
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.data.shape[0], 2 * self.data.shape[1]
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def scale_matrix(self) -> torch.Tensor:
+        """The scales' bytes in the order of the values, uint8 [rows, cols / 32]."""
+        rows, cols = self.shape
+        v = self.scales.view(-(-rows // 128), -(-cols // 128), 32, 4, 4).permute(0, 3, 2, 1, 4)
+        return v.reshape(-(-rows // 128) * 128, -1)[:rows, :cols // 32].contiguous()
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values that the tensor stands for, exact in ``dtype`` (bf16 or fp32)."""
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError("values come back in bf16 or fp32")
+        rows, cols = self.shape
+        out = torch.empty(rows, cols, dtype=dtype, device=self.device)
+        if rows:
+            lib = _lib()
+            with _on(self.device):
+                _native.check(lib, lib.purlin_mx4_dequantize(self.data.data_ptr(), self.scales.data_ptr(), out.data_ptr(), TYPES[dtype], rows, cols, _stream(None)))
+        return out
+
+
+def _check_dense(x: torch.Tensor):
+    if x.dtype not in TYPES:
+        raise TypeError("quantisation takes bf16, fp16 or fp32 values")
+    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
+        raise ValueError("the last dimension must be a multiple of 32")
+    if not (x.is_cuda and x.is_contiguous()):
+        raise ValueError("operands must be contiguous CUDA tensors")
+    if x.data_ptr() % 16:
+        raise ValueError("operands must start on a 16-byte boundary")
+
+
+def _rows(x: torch.Tensor) -> int:
+    return x.numel() // x.shape[-1]
+
+
+def _empty(rows: int, cols: int, device) -> Mx4Tensor:
+    both = torch.empty(rows * cols // 2 + scale_bytes(rows, cols), dtype=torch.uint8, device=device)     # (a row is a multiple of 16 bytes)
+    return Mx4Tensor(both[:rows * cols // 2].view(rows, cols // 2), both[rows * cols // 2:])
+
+
+def quantize_mx4(x: torch.Tensor) -> Mx4Tensor:
+    """``x [..., cols]`` (bf16, fp16 or fp32, contiguous, cols a multiple of 32) as an ``Mx4Tensor`` of its rows. A block's power of two is that of its
+    largest magnitude over 4, at least 2^-127; values are rounded to the nearest of the format, ties to the even code, and above 6 times the power
+    to 6. A block that holds an infinity or a NaN stands for NaNs."""
+    _check_dense(x)
+    rows, cols = _rows(x), x.shape[-1]
+    q = _empty(rows, cols, x.device)
+    if rows:
+        lib = _lib()
+        with _on(x.device):
+            _native.check(lib, lib.purlin_mx4_quantize(x.data_ptr(), TYPES[x.dtype], q.data.data_ptr(), q.scales.data_ptr(), rows, cols, _stream(None)))
+    return q
+
+
+def _product(a: Union[torch.Tensor, Mx4Tensor], w: Mx4Tensor, out: Optional[torch.Tensor], epilogue: int) -> torch.Tensor:
+    if not isinstance(w, Mx4Tensor):
+        raise TypeError("w is an Mx4Tensor (quantize_mx4)")
+    quantised = isinstance(a, Mx4Tensor)
+    if not quantised:
+        _check_dense(a)
+    n, k = w.shape
+    if a.shape[-1] != k or a.device != w.device:
+        raise ValueError("a is [..., K] and w is [N, K], on one device")
+    if n == 0 or n % (32 if epilogue == EPI_SWIGLU else 8):
+        raise ValueError("the SwiGLU epilogue needs N to be a multiple of 32 (16 rows of gate and 16 of up in turn)" if epilogue == EPI_SWIGLU
+                         else "N must be a multiple of 8")
+    rows, cols = (a.shape[0] if quantised else _rows(a)), n // 2 if epilogue == EPI_SWIGLU else n
+    shape = (*a.shape[:-1], cols)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=w.device)
+    elif out.dtype != torch.bfloat16:
+        raise TypeError("out is a bf16 tensor")
+    elif tuple(out.shape) != shape or out.device != w.device or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out is a contiguous tensor of {shape} on the operands' device")
+    if rows == 0:
+        return out
+    lib = _lib()
+    with _on(w.device):
+        if quantised:
+            rc = lib.purlin_mx4_gemm(a.data.data_ptr(), a.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k, epilogue,
+                                     None, _stream(None))
+        else:
+            work = torch.empty(rows * k // 2 + scale_bytes(rows, k), dtype=torch.uint8, device=w.device)
+            at = work.data_ptr()
+            rc = lib.purlin_mx4_linear(a.data_ptr(), TYPES[a.dtype], at, at + rows * k // 2, w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k,
+                                       epilogue, None, _stream(None))
+        _native.check(lib, rc)
+    return out
+
+
+def mx4_gemm(a: Union[torch.Tensor, Mx4Tensor], w: Mx4Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``a @ w.T`` in bf16 for ``a [..., K]``, an ``Mx4Tensor`` or a bf16, fp16 or fp32 tensor that is quantised in the call, and ``w [N, K]``; N a multiple of
+    8. One token or many."""
+    return _product(a, w, out, EPI_STORE)
+
+
+def mx4_gemm_swiglu(a: Union[torch.Tensor, Mx4Tensor], w_gu: Mx4Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``silu(a @ w_gate.T) * (a @ w_up.T)`` for ``w_gu = quantize_mx4(interleave_gate_up(w_gate, w_up))``."""
+    return _product(a, w_gu, out, EPI_SWIGLU)
