@@ -183,25 +183,57 @@ constexpr int kSmemLimit = 227 * 1024;
 PURLIN_D uint32_t instrDescMx4(uint32_t n, uint32_t m, uint32_t half) {
   return (half << 5) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 7) << 27) | (half << 30);
 }
-template <int CTAS> PURLIN_D void mmaMx4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scaleA, uint32_t scaleB, uint32_t accumulate) {
+// The producing and the issuing warp stay whole: all lanes wait and count, and the instructions below are predicated on one lane. In a branch of one
+// lane the compiler has to move every operand into the uniform registers that these instructions read, which made a copy of scales
+// take 45 cycles of the issuing thread instead of 8 and an MMA of few columns 48 instead of 32, with loops of run-time length around them about 90.
+PURLIN_D uint32_t electOne() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
+}
+PURLIN_D bool waitAll(uint32_t bar, uint32_t parity, volatile int* abortWord, uint64_t timeoutNs) {
+  return __all_sync(0xffffffffu, tc::mbarWait(bar, parity, abortWord, timeoutNs)) != 0;
+}
+template <int CTAS> PURLIN_D void mmaMx4(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scaleA, uint32_t scaleB, uint32_t accumulate) {
   if constexpr (CTAS == 2)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                 "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate) : "memory");
+    asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 e, %7, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate), "r"(elected) : "memory");
   else
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate) : "memory");
+    asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 e, %7, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate), "r"(elected) : "memory");
 }
 // 512 bytes of scales (32 rows of 16 bytes) from shared memory into four columns of all four quarters of the TMEM lanes
-template <int CTAS> PURLIN_D void scalesToTmem(uint32_t taddr, uint32_t smemByteAddr) {
-  const uint32_t lo = ((smemByteAddr >> 4) & 0x3FFFu) | (1u << 16), hi = (128u >> 4) | (1u << 14);   // groups of 8 rows, 128 bytes apart, no swizzle
-  const uint64_t desc = uint64_t(lo) | (uint64_t(hi) << 32);
-  if constexpr (CTAS == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+PURLIN_D uint64_t scaleDesc(uint32_t smemByteAddr) {       // groups of 8 rows, 128 bytes apart, no swizzle
+  const uint32_t lo = ((smemByteAddr >> 4) & 0x3FFFu) | (1u << 16), hi = (128u >> 4) | (1u << 14);
+  return uint64_t(lo) | (uint64_t(hi) << 32);
+}
+template <int CTAS> PURLIN_D void scalesToTmem(uint32_t elected, uint32_t taddr, uint64_t desc) {
+  if constexpr (CTAS == 2)
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(elected) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(elected) : "memory");
+}
+template <int CTAS> PURLIN_D void commit(uint32_t elected, uint32_t bar) {      // on this barrier, of both CTAs of a pair
+  if constexpr (CTAS == 2)
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t"
+                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar), "h"(uint16_t(3)), "r"(elected) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(elected) : "memory");
 }
 
 struct alignas(64) Maps { CUtensorMap a, b, sa, sb, c; };
+
+// Scales as [row blocks][rows of 128 bytes, four to a block of 512]: eight of those, of one or two row blocks
+PURLIN_D void loadScales(uint32_t smemDst, const CUtensorMap* map, int y, int rowBlock, uint32_t clusterBarAddress) {
+  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               ::"r"(smemDst), "l"(map), "r"(clusterBarAddress), "r"(0), "r"(y), "r"(rowBlock) : "memory");
+}
+PURLIN_D void loadScalesHere(uint32_t smemDst, const CUtensorMap* map, int y, int rowBlock, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               ::"r"(smemDst), "l"(map), "r"(bar), "r"(0), "r"(y), "r"(rowBlock) : "memory");
+}
 
 // ---- many rows: 256 rows of A x up to 256 rows of W per CTA pair ----
 // One accumulator of 256 columns; the scales of a stage take the columns behind it (two sets in turn). The epilogue gives the accumulator back
@@ -217,7 +249,7 @@ static_assert(kWideSmem <= size_t(kSmemLimit) && kWideStage % 1024 == 0, "the ri
 struct WideParams {
   int M, N, K, bn;                    // bn: columns of a tile, a multiple of 64 (of 128 where its last wave is halved), so they lie in two row blocks of W's scales
   int tilesM, tilesN, items, fullItems;
-  int scaleBlocks;                    // 512-byte blocks of a row block: ceil(K / 128)
+  int boxRows;                        // rows of W to a load: a CTA's half of a tile, or of half a tile where there are such
   uint32_t* status;
   uint64_t timeoutNs;
 };
@@ -269,66 +301,67 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4WideKernel(const __grid_co
   const uint32_t tmemBase = *tmemBaseWord;
   const uint32_t leaderBars = tc::mapToCta(barBase, 0);
   const int kBlocks = (p.K + kBK - 1) / kBK;
-  const int lastBlockA = (p.M - 1) / kScaleRows, lastBlockW = (p.N - 1) / kScaleRows;
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t st = 0, ph = 0;
-      bool ok = true;
-      for (int it = pairIdx; it < p.items && ok; it += numPairs) {
-        const WideItem w = wideItem(p, it);
-        const int half = w.cols / 2, loads = w.cols == p.bn ? 2 : 1, box = p.bn / 4;
-        const int aRow = w.row0 + int(ctaRank) * kBM, bRow = w.col0 + int(ctaRank) * half;
-        // Row blocks of the scales: this CTA's rows of A, all columns of the tile. Blocks past the last one (their values are zeros and their
-        // results are not stored) take the last one's.
-        const int sa = min(aRow / kScaleRows, lastBlockA), sb = w.col0 / kScaleRows, sbs = (w.col0 + w.cols - 1) / kScaleRows - sb + 1;
-        const uint32_t bytes = uint32_t(2 * (kABytes + half * 128 + (1 + sbs) * kScaleStage));
-        for (int kb = 0; kb < kBlocks; ++kb) {
-          ok = tc::mbarWait(emptyBar(st), ph ^ 1, abortWord, p.timeoutNs);
-          if (!ok) { skinny::recordTimeout(p.status, 1, it, kb); break; }
-          const uint32_t sA = base + st * kWideStage, sB = sA + kABytes, sS = sB + kMaxCols / 2 * 128;
-          const uint32_t full = leaderBars + 8u * st;
+    const uint32_t elected = electOne();
+    uint32_t st = 0, ph = 0;
+    bool ok = true;
+    for (int it = pairIdx; it < p.items && ok; it += numPairs) {
+      const WideItem w = wideItem(p, it);
+      const int half = w.cols / 2;
+      const int aRow = w.row0 + int(ctaRank) * kBM, bRow = w.col0 + int(ctaRank) * half;
+      // row blocks of the scales: this CTA's rows of A, all columns of the tile (two blocks; what lies past the last one reads as zero)
+      const int sa = aRow / kScaleRows, sb = w.col0 / kScaleRows;
+      const uint32_t bytes = uint32_t(2 * (kABytes + half * 128 + 3 * kScaleStage));
+      for (int kb = 0; kb < kBlocks; ++kb) {
+        ok = waitAll(emptyBar(st), ph ^ 1, abortWord, p.timeoutNs);
+        if (!ok) { if (elected) skinny::recordTimeout(p.status, 1, it, kb); break; }
+        const uint32_t sA = base + st * kWideStage, sB = sA + kABytes, sS = sB + kMaxCols / 2 * 128;
+        const uint32_t full = leaderBars + 8u * st;
+        if (elected) {
           if (ctaRank == 0) tc::mbarExpectTx(fullBar(st), bytes);
           tc::tmaLoad2dPair(sA, &maps.a, kb * 128, aRow, full);
-          for (int i = 0; i < loads; ++i) tc::tmaLoad2dPair(sB + uint32_t(i * box * 128), &maps.b, kb * 128, bRow + i * box, full);
-          tc::tmaLoad2dPair(sS, &maps.sa, 0, (sa * p.scaleBlocks + 2 * kb) * 4, full);
-          for (int i = 0; i < sbs; ++i) tc::tmaLoad2dPair(sS + uint32_t((1 + i) * kScaleStage), &maps.sb, 0, (min(sb + i, lastBlockW) * p.scaleBlocks + 2 * kb) * 4, full);
-          if (++st == kWideStages) { st = 0; ph ^= 1; }
+          tc::tmaLoad2dPair(sB, &maps.b, kb * 128, bRow, full);
+          if (half > p.boxRows) tc::tmaLoad2dPair(sB + uint32_t(p.boxRows * 128), &maps.b, kb * 128, bRow + p.boxRows, full);
+          loadScales(sS, &maps.sa, 8 * kb, sa, full);
+          loadScales(sS + kScaleStage, &maps.sb, 8 * kb, sb, full);
         }
+        __syncwarp();
+        if (++st == kWideStages) { st = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && ctaRank == 0) {
+    if (ctaRank == 0) {
+      const uint32_t elected = electOne();
       uint32_t st = 0, ph = 0, use = 0, set = 0;
       bool ok = true;
-      const uint64_t descA0 = tc::smemDescSw128(base), descB0 = tc::smemDescSw128(base + kABytes);
+      const uint64_t descA0 = tc::smemDescSw128(base), descB0 = tc::smemDescSw128(base + kABytes), descS0 = scaleDesc(base + kABytes + kMaxCols / 2 * 128);
       for (int it = pairIdx; it < p.items && ok; it += numPairs, ++use) {
         const WideItem w = wideItem(p, it);
-        const uint32_t sbs = uint32_t((w.col0 + w.cols - 1) / kScaleRows - w.col0 / kScaleRows + 1), shift = uint32_t(w.col0 % kScaleRows / 32);
+        const uint32_t shift = uint32_t(w.col0 % kScaleRows / 32);
         const uint32_t idesc = instrDescMx4(uint32_t(w.cols), 2 * kBM, 0), idescHigh = instrDescMx4(uint32_t(w.cols), 2 * kBM, 1);
-        ok = tc::mbarWait(tmemEmpty, (use & 1) ^ 1, abortWord, p.timeoutNs);
-        if (!ok) { skinny::recordTimeout(p.status, 2, it, 0); break; }
+        ok = waitAll(tmemEmpty, (use & 1) ^ 1, abortWord, p.timeoutNs);
+        if (!ok) { if (elected) skinny::recordTimeout(p.status, 2, it, 0); break; }
         for (int kb = 0; kb < kBlocks; ++kb, set ^= 1) {
-          ok = tc::mbarWait(fullBar(st), ph, abortWord, p.timeoutNs);
-          if (!ok) { skinny::recordTimeout(p.status, 3, it, kb); break; }
+          ok = waitAll(fullBar(st), ph, abortWord, p.timeoutNs);
+          if (!ok) { if (elected) skinny::recordTimeout(p.status, 3, it, kb); break; }
           tc::fenceAfterThreadSync();
-          // 64 of k to an MMA, 128 to a block of scales; what lies past K is neither scaled nor multiplied
-          const int left = p.K - kb * kBK, steps = min((left + 63) / 64, 4), blocks = min((left + 127) / 128, 2);
-          const uint32_t sS = base + st * kWideStage + kABytes + kMaxCols / 2 * 128;
+          const uint64_t off = uint64_t(st * (kWideStage >> 4)), da = descA0 + off, db = descB0 + off, ds = descS0 + off;
           const uint32_t scaleA = tmemBase + kScaleTmem + set * kScaleSet, scaleB = scaleA + 8;
-          for (int q = 0; q < blocks; ++q) {
-            scalesToTmem<2>(scaleA + 4u * q, sS + uint32_t(q * kScaleBytes));
-            for (uint32_t i = 0; i < sbs; ++i) scalesToTmem<2>(scaleB + 8u * q + 4u * i, sS + (1 + i) * kScaleStage + uint32_t(q * kScaleBytes));
-          }
-          const uint64_t da = descA0 + uint64_t(st * (kWideStage >> 4)), db = descB0 + uint64_t(st * (kWideStage >> 4));
+          // [scales of A: two blocks][of the first 128 columns: two blocks][of the next 128], 512 bytes each
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (k < steps)
-              mmaMx4<2>(tmemBase, da + 2 * k, db + 2 * k, k & 1 ? idescHigh : idesc, scaleA + 4u * (k / 2), scaleB + 8u * (k / 2) + shift, uint32_t((kb | k) != 0));
-          tc::mmaCommitPairs(emptyBar(st), 3u);
+          for (uint32_t q = 0; q < 2; ++q) {
+            scalesToTmem<2>(elected, scaleA + 4 * q, ds + 32 * q);
+            scalesToTmem<2>(elected, scaleB + 8 * q, ds + 64 + 32 * q);
+            scalesToTmem<2>(elected, scaleB + 8 * q + 4, ds + 128 + 32 * q);
+          }
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k)      // (past K values and scales are zeros)
+            mmaMx4<2>(elected, tmemBase, da + 2 * k, db + 2 * k, k & 1 ? idescHigh : idesc, scaleA + 4 * (k / 2), scaleB + 8 * (k / 2) + shift, uint32_t(kb != 0 || k != 0));
+          commit<2>(elected, emptyBar(st));
           if (++st == kWideStages) { st = 0; ph ^= 1; }
         }
-        if (ok) tc::mmaCommitPairs(tmemFull, 3u);
+        if (ok) commit<2>(elected, tmemFull);
       }
     }
   } else {
@@ -406,7 +439,6 @@ constexpr int kFewThreads = skinny::kThreads, kFewTokens = 128, kWRows = 128;
 struct FewParams {
   int N, K, tokens, cols;              // cols: columns of the MMA, tokens rounded up to 16
   int stages, tmemCols, ahead;
-  int scaleBlocks;
   __nv_bfloat16* C;
   int ldc;
   uint32_t* status;
@@ -462,47 +494,46 @@ __global__ void __launch_bounds__(kFewThreads, 2) mx4FewKernel(const __grid_cons
   bool ok = true;
   uint32_t st = 0, ph = 0;
   if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t bytes = stageBytes;
-      for (int kb = kBegin; kb < kEnd && ok; ++kb) {
-        ok = tc::mbarWait(emptyBar(st), ph ^ 1, abortWord, p.timeoutNs);
-        if (!ok) { skinny::recordTimeout(p.status, 1, tile, kb); break; }
-        const uint32_t sW = base + st * stageBytes, sX = sW + kABytes, sS = sX + uint32_t(p.cols * 128);
-        tc::mbarExpectTx(fullBar(st), bytes);
+    const uint32_t elected = electOne();
+    for (int kb = kBegin; kb < kEnd && ok; ++kb) {
+      ok = waitAll(emptyBar(st), ph ^ 1, abortWord, p.timeoutNs);
+      if (!ok) { if (elected) skinny::recordTimeout(p.status, 1, tile, kb); break; }
+      const uint32_t sW = base + st * stageBytes, sX = sW + kABytes, sS = sX + uint32_t(p.cols * 128);
+      if (elected) {
+        tc::mbarExpectTx(fullBar(st), stageBytes);
         tc::tmaLoad2d(sW, &maps.a, kb * 128, tile * kWRows, fullBar(st));
-        tc::tmaLoad2d(sS, &maps.sa, 0, (tile * p.scaleBlocks + 2 * kb) * 4, fullBar(st));
+        loadScalesHere(sS, &maps.sa, 8 * kb, tile, fullBar(st));
         tc::tmaLoad2d(sX, &maps.b, kb * 128, 0, fullBar(st));
-        tc::tmaLoad2d(sS + kScaleStage, &maps.sb, 0, 2 * kb * 4, fullBar(st));
-        if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
+        loadScalesHere(sS + kScaleStage, &maps.sb, 8 * kb, 0, fullBar(st));
       }
+      __syncwarp();
+      if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = instrDescMx4(uint32_t(p.cols), kWRows, 0), idescHigh = instrDescMx4(uint32_t(p.cols), kWRows, 1);
-      const uint64_t descW = tc::smemDescSw128(base), descX = tc::smemDescSw128(base + kABytes);
-      const uint32_t scales = tmemBase + uint32_t((p.cols + 31) / 32 * 32);
-      uint32_t set = 0;
-      for (int kb = kBegin; kb < kEnd && ok; ++kb, set ^= 1) {
-        ok = tc::mbarWait(fullBar(st), ph, abortWord, p.timeoutNs);
-        if (!ok) { skinny::recordTimeout(p.status, 3, tile, kb); break; }
-        tc::fenceAfterThreadSync();
-        const int left = p.K - kb * kBK, steps = min((left + 63) / 64, 4), blocks = min((left + 127) / 128, 2);
-        const uint32_t sS = base + st * stageBytes + kABytes + uint32_t(p.cols * 128);
-        const uint32_t scaleW = scales + set * 16, scaleX = scaleW + 8;
-        for (int q = 0; q < blocks; ++q) {
-          scalesToTmem<1>(scaleW + 4u * q, sS + uint32_t(q * kScaleBytes));
-          scalesToTmem<1>(scaleX + 4u * q, sS + kScaleStage + uint32_t(q * kScaleBytes));
-        }
-        const uint64_t step = uint64_t(st * (stageBytes >> 4));
+    const uint32_t elected = electOne();
+    const uint32_t idesc = instrDescMx4(uint32_t(p.cols), kWRows, 0), idescHigh = instrDescMx4(uint32_t(p.cols), kWRows, 1);
+    const uint64_t descW = tc::smemDescSw128(base), descX = tc::smemDescSw128(base + kABytes), descS = scaleDesc(base + kABytes + uint32_t(p.cols * 128));
+    const uint32_t scales = tmemBase + uint32_t((p.cols + 31) / 32 * 32);
+    uint32_t set = 0;
+    for (int kb = kBegin; kb < kEnd && ok; ++kb, set ^= 1) {
+      ok = waitAll(fullBar(st), ph, abortWord, p.timeoutNs);
+      if (!ok) { if (elected) skinny::recordTimeout(p.status, 3, tile, kb); break; }
+      tc::fenceAfterThreadSync();
+      const uint64_t off = uint64_t(st * (stageBytes >> 4));
+      const uint32_t scaleW = scales + set * 16, scaleX = scaleW + 8;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k < steps)
-            mmaMx4<1>(tmemBase, descW + step + 2 * k, descX + step + 2 * k, k & 1 ? idescHigh : idesc, scaleW + 4u * (k / 2), scaleX + 4u * (k / 2), uint32_t(kb != kBegin || k != 0));
-        tc::mmaCommit(emptyBar(st));
-        if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
+      for (uint32_t q = 0; q < 2; ++q) {
+        scalesToTmem<1>(elected, scaleW + 4 * q, descS + off + 32 * q);
+        scalesToTmem<1>(elected, scaleX + 4 * q, descS + off + 64 + 32 * q);
       }
-      if (ok) tc::mmaCommit(accFull);
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)          // (past K values and scales are zeros)
+        mmaMx4<1>(elected, tmemBase, descW + off + 2 * k, descX + off + 2 * k, k & 1 ? idescHigh : idesc, scaleW + 4 * (k / 2), scaleX + 4 * (k / 2),
+                  uint32_t(kb != kBegin || k != 0));
+      commit<1>(elected, emptyBar(st));
+      if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
     }
+    if (ok) commit<1>(elected, accFull);
   } else {
     // ---- this CTA's partial tile: TMEM (lane = row of W, column = token) -> shared memory [token][row of W] ----
     const int quarter = warp & 3;
@@ -600,14 +631,15 @@ int launchRows(void (*kernel)(A...), int64_t total, const Device& dev, cudaStrea
   return launched(cudaLaunchKernelEx(&cfg, kernel, args...)) ? 0 : 1;
 }
 
-// rows of 128 bytes without a swizzle, eight of them (the scales of 128 rows x 256 columns) to a box
-bool scaleMap(CUtensorMap* map, const void* ptr, uint64_t bytes) {
+// the scales of 128 rows x 256 columns, of `rowBlocks` row blocks, to a box; past the edges zeros
+bool scaleMap(CUtensorMap* map, const void* ptr, int rows, int cols, int rowBlocks) {
   const TensorMapEncodeFn fn = tensorMapEncodeFn();
   if (!fn) { setError("cuTensorMapEncodeTiled is not available from this driver"); return false; }
   if (reinterpret_cast<uintptr_t>(ptr) % 16) { setError("TMA operands need 16-byte aligned base and row pitch"); return false; }
-  const cuuint64_t dims[2] = {128, bytes / 128}, strides[1] = {128};
-  const cuuint32_t box[2] = {128, kScaleStage / 128}, elem[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+  const uint64_t blocks = uint64_t(cols + kScaleCols - 1) / kScaleCols;
+  const cuuint64_t dims[3] = {128, blocks * 4, uint64_t(rows + kScaleRows - 1) / kScaleRows}, strides[2] = {128, blocks * kScaleBytes};
+  const cuuint32_t box[3] = {128, kScaleStage / 128, uint32_t(rowBlocks)}, elem[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) { setError("cuTensorMapEncodeTiled failed with code " + std::to_string(int(r))); return false; }
   return true;
@@ -639,7 +671,7 @@ int launchFew(const void* aData, const void* aScales, const void* wData, const v
   const int outCols = swiglu ? N / 2 : N;
   if (reinterpret_cast<uintptr_t>(C) % 16) { setError("TMA operands need 16-byte aligned base and row pitch"); return 1; }
   FewParams p{};
-  p.N = N; p.K = K; p.tokens = M; p.cols = (M + 15) / 16 * 16; p.scaleBlocks = (K + kScaleCols - 1) / kScaleCols;
+  p.N = N; p.K = K; p.tokens = M; p.cols = (M + 15) / 16 * 16;
   p.C = static_cast<__nv_bfloat16*>(C); p.ldc = outCols; p.status = status; p.timeoutNs = 2ull * 1000 * 1000 * 1000;
   const int tiles = (N + kWRows - 1) / kWRows, kBlocks = (K + kBK - 1) / kBK;
   // k is cut while that brings more CTAs to work (two to an SM) and leaves each at least four k-blocks
@@ -654,7 +686,7 @@ int launchFew(const void* aData, const void* aScales, const void* wData, const v
   Maps maps{};
   if (!makeTensorMap(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, wData, uint64_t(N), uint64_t(K) / 2, uint64_t(K) / 2, kWRows) ||
       !makeTensorMap(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, aData, uint64_t(M), uint64_t(K) / 2, uint64_t(K) / 2, uint32_t(p.cols)) ||
-      !scaleMap(&maps.sa, wScales, scaleBytes(N, K)) || !scaleMap(&maps.sb, aScales, scaleBytes(M, K))) return 1;
+      !scaleMap(&maps.sa, wScales, N, K, 1) || !scaleMap(&maps.sb, aScales, M, K, 1)) return 1;
   auto kernel = swiglu ? mx4FewKernel<true> : mx4FewKernel<false>;
   static bool done[64][2] = {};
   if (!optIn(reinterpret_cast<const void*>(kernel), done[dev.index][swiglu])) return 1;
@@ -692,7 +724,7 @@ int launchWide(const void* aData, const void* aScales, const void* wData, const 
     pairs = n;
   }
   WideParams p{};
-  p.M = M; p.N = N; p.K = K; p.scaleBlocks = (K + kScaleCols - 1) / kScaleCols; p.status = status; p.timeoutNs = 2ull * 1000 * 1000 * 1000;
+  p.M = M; p.N = N; p.K = K; p.status = status; p.timeoutNs = 2ull * 1000 * 1000 * 1000;
   p.tilesM = (M + 2 * kBM - 1) / (2 * kBM);
   // the width that is expected to take least: a tile costs its columns and about 48 columns' worth besides (fill, drain, the loads of A)
   double least = 1e30;
@@ -705,13 +737,14 @@ int launchWide(const void* aData, const void* aScales, const void* wData, const 
       p.bn = bn; p.tilesN = tilesN;
       p.fullItems = halved ? tiles - rest : tiles;
       p.items = halved ? p.fullItems + 2 * rest : tiles;
+      p.boxRows = halved ? bn / 4 : bn / 2;
     }
   }
   const int outCols = swiglu ? N / 2 : N;
   Maps maps{};
   if (!makeTensorMap(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, aData, uint64_t(M), uint64_t(K) / 2, uint64_t(K) / 2, kBM) ||
-      !makeTensorMap(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, wData, uint64_t(N), uint64_t(K) / 2, uint64_t(K) / 2, uint32_t(p.bn / 4)) ||
-      !scaleMap(&maps.sa, aScales, scaleBytes(M, K)) || !scaleMap(&maps.sb, wScales, scaleBytes(N, K)) ||
+      !makeTensorMap(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, wData, uint64_t(N), uint64_t(K) / 2, uint64_t(K) / 2, uint32_t(p.boxRows)) ||
+      !scaleMap(&maps.sa, aScales, M, K, 1) || !scaleMap(&maps.sb, wScales, N, K, 2) ||
       !(swiglu ? narrowOutputMap(&maps.c, C, uint64_t(M), uint64_t(outCols))
                : makeTensorMap(&maps.c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, C, uint64_t(M), uint64_t(outCols) * 2, uint64_t(outCols) * 2, 32))) return 1;
   cfg.gridDim = dim3(unsigned(2 * std::min(pairs, p.items))); cfg.numAttrs = 2;
