@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <mutex>
 #include <string>
+#include <type_traits>
 
 #include "purlin/gated_ffn.h"
 #include "purlin/gemm.h"
@@ -36,7 +37,6 @@ using namespace purlin;
 namespace {
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kABytes = kBM * kBK * 2;          // 16 KiB
 constexpr int kBoxBytes = 64 * 128;             // a box of 64 x 64 of an operand whose rows or columns are contiguous
 constexpr int kAccStride = 256, kTmemCols = 512;
 constexpr int kEpiWarps = 8, kThreads = 32 * (2 + kEpiWarps);
@@ -51,19 +51,29 @@ static_assert(8 * (2 * kMaxStages + 4) + 8 <= kBarrierBytes, "the barriers, the 
 
 enum { kStore = 0, kGate = 1, kGateGrad = 2 };
 
-struct Params {
-  int M, N, K, bn, stages, aBytes;       // aBytes: of one block of A in a stage (fewer than 128 rows where there are fewer)
-  int tilesM, tilesN;
-  int items, fullItems;                  // tiles [0, fullItems) whole, then the remaining ones as halves of one accumulator
-  __nv_bfloat16* C;                      // output, or dZ
-  int ldc;
+// One product. A launch has one, or the three gradients, which need one another as little as their tiles do.
+struct alignas(64) Group {
+  CUtensorMap a, b, c;
+  int M, N, K, tilesM, tilesN;
+  int aMn;                               // m is contiguous in A (k otherwise)
+  int aBytes;                            // that one block of A brings into a stage: fewer than 128 rows of it where there are fewer
+};
+// Tiles [start, start + count) of a group (with `halves` their accumulators one by one, 2 * count of them) in turn over `pairs` CTA pairs (or CTAs)
+// from number `first` on, wrapping around.
+struct Segment { int group, start, count, first, pairs, halves; };
+constexpr int kMaxGroups = 3, kMaxSegments = 3 * kMaxGroups;
+
+struct alignas(64) Params {
+  Group g[kMaxGroups];
+  Segment seg[kMaxSegments];
+  int segments;
+  int bn, stages, aBytes;                // aBytes: room of one block of A in a stage
   uint4* saved;                          // pre-activations: written by kGate (unless null), read by kGateGrad
   int savedCols;                         // its 32-column blocks per row block
   int activation;
   uint32_t* status;
   uint64_t timeoutNs;
 };
-struct alignas(64) Maps { CUtensorMap a, b, c; };
 
 PURLIN_D float sigmoidOf(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 // act(g) = g sigmoid(s(g)): s = g (silu), s = 2 sqrt(2 / pi) (g + 0.044715 g^3) (gelu with the tanh). Past |g| = 16 the sigmoid is 0 or 1
@@ -124,26 +134,73 @@ PURLIN_D void gateGrad(int activation, const uint32_t (&r)[32], const uint32_t (
   }
 }
 
+// The producing and the issuing warp stay whole, their instructions are predicated on one lane: in a branch of one lane every operand of an
+// MMA would have to be moved into uniform registers first.
+PURLIN_D uint32_t electOne() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
+}
+PURLIN_D bool waitAll(uint32_t bar, uint32_t parity, volatile int* abortWord, uint64_t timeoutNs) {
+  return __all_sync(0xffffffffu, tc::mbarWait(bar, parity, abortWord, timeoutNs)) != 0;
+}
+template <int CTAS> PURLIN_D void mma(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CTAS == 2)
+    asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
+}
+template <int CTAS> PURLIN_D void commit(uint32_t elected, uint32_t bar) {      // on this barrier of every CTA of the tile
+  if constexpr (CTAS == 2)
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t"
+                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar), "h"(uint16_t(3)), "r"(elected) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(elected) : "memory");
+}
+
 // Tile t -> (row block, column block), rows fastest inside bands of row blocks: the tiles in flight share operands in L2
 constexpr int kBand = 8;
-PURLIN_D void tileCoord(const Params& p, int t, int& mIdx, int& nIdx) {
-  const int perBand = kBand * p.tilesN, band = t / perBand, within = t - band * perBand, first = band * kBand;
-  const int rows = min(p.tilesM - first, kBand);
+PURLIN_D void tileCoord(const Group& g, int t, int& mIdx, int& nIdx) {
+  const int perBand = kBand * g.tilesN, band = t / perBand, within = t - band * perBand, first = band * kBand;
+  const int rows = min(g.tilesM - first, kBand);
   mIdx = first + within % rows;
   nIdx = within / rows;
 }
-struct Item { int tile, first, count; };     // accumulators [first, first + count) of a tile
-template <int ACCS> PURLIN_D Item itemOf(const Params& p, int i) {
-  if (ACCS == 1 || i < p.fullItems) return Item{i, 0, ACCS};
-  const int j = i - p.fullItems;
-  return Item{p.fullItems + (j >> 1), j & 1, 1};
+// first row of the pair's accumulators, first column, number of accumulators
+struct Item { int group, tile, row, col, count; };
+// The work of pair `idx` of `units`, in the order in which all warps walk it; body returns false to stop.
+template <int CTAS, int ACCS, typename F> PURLIN_D void forItems(const Params& p, int idx, int units, F&& body) {
+  for (int s = 0; s < p.segments; ++s) {
+    const Segment& seg = p.seg[s];
+    const Group& g = p.g[seg.group];
+    const int at = idx - seg.first + (idx < seg.first ? units : 0);
+    if (at >= seg.pairs) continue;
+    const int n = ACCS == 2 && seg.halves ? 2 * seg.count : seg.count;
+    for (int i = at; i < n; i += seg.pairs) {
+      Item m;
+      int mIdx, nIdx, first = 0;
+      m.group = seg.group;
+      m.tile = seg.start + (ACCS == 2 && seg.halves ? i >> 1 : i);
+      tileCoord(g, m.tile, mIdx, nIdx);
+      m.count = 1;
+      if constexpr (ACCS == 2) {
+        if (seg.halves) first = i & 1;
+        else m.count = (mIdx * ACCS + 1) * CTAS * kBM < g.M ? 2 : 1;      // rows of the last tile that end in its first accumulator
+      }
+      m.row = (mIdx * ACCS + first) * CTAS * kBM;
+      m.col = nIdx * p.bn;
+      if (m.row < g.M && !body(m)) return;
+    }
+  }
 }
 
 // CTAS = 2: a cluster of two CTAs owns a tile: each loads its 128 rows of A per accumulator and its half of B's columns, CTA 0 issues one
 // 256-row MMA for the pair. ACCS = 2: a tile is two accumulators tall; they share B, and their MMAs alternate (an MMA waits for the one before
 // into the same columns). ACCS = 1: tiles alternate between the two accumulators, the epilogue of one runs under the MMAs of the next.
-template <bool A_MN, bool B_MN, int EPI, int CTAS, int ACCS>
-__global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+template <bool B_MN, int EPI, int CTAS, int ACCS>
+__global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__ Params p) {
   extern __shared__ unsigned char smemRaw[];
   const uint32_t rawAddr = tc::smemAddr(smemRaw);
   const uint32_t base = (rawAddr + 1023u) & ~1023u;
@@ -170,8 +227,8 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
     for (int a = 0; a < 2; ++a) { tc::mbarInit(tmemFullBar(a), 1); tc::mbarInit(tmemEmptyBar(a), kEpiWarps / 2 * CTAS); }
     *abortWord = 0;
     tc::mbarFenceInit();
-    tc::tmaPrefetchDescriptor(&maps.a);
-    tc::tmaPrefetchDescriptor(&maps.b);
+    tc::tmaPrefetchDescriptor(&p.g[0].a);
+    tc::tmaPrefetchDescriptor(&p.g[0].b);
   }
   if (warp == 1) {
     if constexpr (CTAS == 2) { tc::tmemAllocPair(tc::smemAddr(words), kTmemCols); tc::tmemRelinquishPair(); }
@@ -184,95 +241,103 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
   tc::gridLaunchDependents();
   const uint32_t tmemBase = *tmemBaseWord;
   const uint32_t leaderBars = CTAS == 2 ? tc::mapToCta(barBase, 0) : barBase;
-  const int kBlocks = (p.K + kBK - 1) / kBK;
+  constexpr bool kAnyA = EPI == kStore;       // A's order goes by the product (k is contiguous in the others)
 
   if (warp == 0) {
     // ---- TMA producer ----
-    if (lane == 0) {
-      uint32_t st = 0, ph = 0;
-      bool ok = true;
-      for (int it = pairIdx; it < p.items && ok; it += numPairs) {
-        const Item item = itemOf<ACCS>(p, it);
-        int mIdx, nIdx;
-        tileCoord(p, item.tile, mIdx, nIdx);
-        const int aRow = ((mIdx * ACCS + item.first) * CTAS + int(ctaRank)) * kBM, bRow = nIdx * p.bn + int(ctaRank) * bnLocal;
-        for (int kb = 0; kb < kBlocks; ++kb) {
-          ok = tc::mbarWait(emptyBar(st), ph ^ 1, abortWord, p.timeoutNs);
-          if (!ok) { skinny::recordTimeout(p.status, 1, item.tile, kb); break; }
+    const uint32_t elected = electOne();
+    uint32_t st = 0, ph = 0;
+    forItems<CTAS, ACCS>(p, pairIdx, numPairs, [&](const Item& m) {
+      const Group& g = p.g[m.group];
+      const int aRow = m.row + int(ctaRank) * kBM, bRow = m.col + int(ctaRank) * bnLocal, kBlocks = (g.K + kBK - 1) / kBK;
+      const bool aMn = kAnyA && g.aMn;
+      const uint32_t bytes = uint32_t(CTAS * (m.count * g.aBytes + bBytes));
+      for (int kb = 0; kb < kBlocks; ++kb) {
+        const bool ok = waitAll(emptyBar(st), ph ^ 1, abortWord, p.timeoutNs);
+        if (!ok) { if (elected) skinny::recordTimeout(p.status, 1, m.tile, kb); return false; }
+        if (elected) {
           const uint32_t sA = base + st * stageBytes, sB = sA + uint32_t(ACCS * p.aBytes);
           const uint32_t full = leaderBars + 8u * st;                   // both CTAs' bytes are credited to CTA 0's barrier
-          if (CTAS == 1 || ctaRank == 0) tc::mbarExpectTx(fullBar(st), uint32_t(CTAS * (item.count * p.aBytes + bBytes)));
+          if (CTAS == 1 || ctaRank == 0) tc::mbarExpectTx(fullBar(st), bytes);
           auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
             if constexpr (CTAS == 2) tc::tmaLoad2dPair(dst, map, x, y, full);
             else tc::tmaLoad2d(dst, map, x, y, fullBar(st));
           };
 #pragma unroll
           for (int a = 0; a < ACCS; ++a) {
-            if (a >= item.count) break;
+            if (a >= m.count) break;
             const int row = aRow + a * CTAS * kBM;
-            if constexpr (A_MN) {
-              load(sA + uint32_t(a * kABytes), &maps.a, row, kb * kBK);
-              load(sA + uint32_t(a * kABytes + kBoxBytes), &maps.a, row + 64, kb * kBK);
+            const uint32_t dst = sA + uint32_t(a * p.aBytes);
+            if (aMn) {
+              load(dst, &g.a, row, kb * kBK);
+              load(dst + kBoxBytes, &g.a, row + 64, kb * kBK);
             } else {
-              load(sA + uint32_t(a * p.aBytes), &maps.a, kb * kBK, row);
+              load(dst, &g.a, kb * kBK, row);
             }
           }
           if constexpr (B_MN) {
-            for (int j = 0; j < bnLocal / 64; ++j) load(sB + uint32_t(j * kBoxBytes), &maps.b, bRow + 64 * j, kb * kBK);
+            for (int j = 0; j < bnLocal / 64; ++j) load(sB + uint32_t(j * kBoxBytes), &g.b, bRow + 64 * j, kb * kBK);
           } else {
-            load(sB, &maps.b, kb * kBK, bRow);
+            load(sB, &g.b, kb * kBK, bRow);
           }
-          if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
         }
+        __syncwarp();
+        if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
       }
-    }
+      return true;
+    });
   } else if (warp == 1) {
     // ---- MMA issuer (CTA 0 of a pair) ----
-    if (lane == 0 && ctaRank == 0) {
-      const uint32_t idesc = tc::instrDescBf16(uint32_t(p.bn), uint32_t(kBM * CTAS)) | (A_MN ? tc::kInstrDescAMnMajor : 0u) | (B_MN ? tc::kInstrDescBMnMajor : 0u);
-      const uint64_t descA0 = A_MN ? tc::smemDescSw128MnMajor(base) : tc::smemDescSw128(base);
+    if (ctaRank == 0) {
+      const uint32_t elected = electOne();
       const uint32_t bBase = base + uint32_t(ACCS * p.aBytes);
       const uint64_t descB0 = B_MN ? tc::smemDescSw128MnMajor(bBase) : tc::smemDescSw128(bBase);
-      constexpr uint32_t kStepA = A_MN ? 128 : 2, kStepB = B_MN ? 128 : 2;        // 16 of k, in units of 16 bytes
+      constexpr uint32_t kStepK = 2, kStepMn = 128;                     // 16 of k, in units of 16 bytes
+      constexpr uint32_t kStepB = B_MN ? kStepMn : kStepK;
       const uint32_t stageStep = stageBytes >> 4, accStep = uint32_t(p.aBytes) >> 4;
       uint32_t st = 0, ph = 0, accIt = 0, use0 = 0, use1 = 0;
-      bool ok = true;
-      auto commit = [&](uint32_t bar) {                                 // on this barrier of every CTA of the tile
-        if constexpr (CTAS == 2) tc::mmaCommitPairs(bar, 3u);
-        else tc::mmaCommit(bar);
-      };
-      for (int it = pairIdx; it < p.items && ok; it += numPairs, ++accIt) {
-        const Item item = itemOf<ACCS>(p, it);
+      forItems<CTAS, ACCS>(p, pairIdx, numPairs, [&](const Item& m) {
+        const Group& g = p.g[m.group];
+        const int kBlocks = (g.K + kBK - 1) / kBK;
         const int a0 = ACCS == 1 ? int(accIt & 1) : 0;
-        const bool two = ACCS == 2 && item.count == 2;
-        ok = tc::mbarWait(tmemEmptyBar(a0), ((a0 ? use1 : use0) & 1) ^ 1, abortWord, p.timeoutNs);
-        if (ok && two) ok = tc::mbarWait(tmemEmptyBar(1), (use1 & 1) ^ 1, abortWord, p.timeoutNs);
-        if (!ok) { skinny::recordTimeout(p.status, 2, item.tile, 0); break; }
+        const bool two = ACCS == 2 && m.count == 2;
+        bool ok = waitAll(tmemEmptyBar(a0), ((a0 ? use1 : use0) & 1) ^ 1, abortWord, p.timeoutNs);
+        if (ok && two) ok = waitAll(tmemEmptyBar(1), (use1 & 1) ^ 1, abortWord, p.timeoutNs);
+        if (!ok) { if (elected) skinny::recordTimeout(p.status, 2, m.tile, 0); return false; }
         const uint32_t d0 = tmemBase + uint32_t(a0) * kAccStride, d1 = tmemBase + kAccStride;
-        for (int kb = 0; kb < kBlocks; ++kb) {
-          ok = tc::mbarWait(fullBar(st), ph, abortWord, p.timeoutNs);
-          if (!ok) { skinny::recordTimeout(p.status, 3, item.tile, kb); break; }
-          tc::fenceAfterThreadSync();
-          const uint64_t da = descA0 + uint64_t(st * stageStep), db = descB0 + uint64_t(st * stageStep);
+        auto mainLoop = [&](auto both, auto order) {
+          constexpr bool aMn = decltype(order)::value;
+          constexpr uint32_t kStepA = aMn ? kStepMn : kStepK;
+          const uint32_t idesc = tc::instrDescBf16(uint32_t(p.bn), uint32_t(kBM * CTAS)) | (aMn ? tc::kInstrDescAMnMajor : 0u) | (B_MN ? tc::kInstrDescBMnMajor : 0u);
+          const uint64_t descA0 = aMn ? tc::smemDescSw128MnMajor(base) : tc::smemDescSw128(base);
+          for (int kb = 0; kb < kBlocks; ++kb) {
+            ok = waitAll(fullBar(st), ph, abortWord, p.timeoutNs);
+            if (!ok) { if (elected) skinny::recordTimeout(p.status, 3, m.tile, kb); return; }
+            tc::fenceAfterThreadSync();
+            const uint64_t off = uint64_t(st * stageStep), da = descA0 + off, db = descB0 + off;
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k) {
-            const uint32_t accumulate = uint32_t((kb | k) != 0);
-            if constexpr (CTAS == 2) {
-              tc::mmaPair(d0, da + kStepA * k, db + kStepB * k, idesc, accumulate);
-              if constexpr (ACCS == 2) { if (two) tc::mmaPair(d1, da + accStep + kStepA * k, db + kStepB * k, idesc, accumulate); }
-            } else {
-              tc::mma(d0, da + kStepA * k, db + kStepB * k, idesc, accumulate);
+            for (int k = 0; k < kBK / 16; ++k) {
+              const uint32_t accumulate = uint32_t(kb != 0 || k != 0);
+              mma<CTAS>(elected, d0, da + kStepA * k, db + kStepB * k, idesc, accumulate);
+              if constexpr (decltype(both)::value) mma<CTAS>(elected, d1, da + accStep + kStepA * k, db + kStepB * k, idesc, accumulate);
             }
+            commit<CTAS>(elected, emptyBar(st));
+            if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
           }
-          commit(emptyBar(st));
-          if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
-        }
-        if (ok) {
-          commit(tmemFullBar(a0));
-          if (a0) ++use1; else ++use0;
-          if (two) { commit(tmemFullBar(1)); ++use1; }
-        }
-      }
+        };
+        auto inOrder = [&](auto both) {
+          if constexpr (kAnyA) { if (g.aMn) mainLoop(both, std::true_type{}); else mainLoop(both, std::false_type{}); }
+          else mainLoop(both, std::false_type{});
+        };
+        if constexpr (ACCS == 2) { if (two) inOrder(std::true_type{}); else inOrder(std::false_type{}); }
+        else inOrder(std::false_type{});
+        if (!ok) return false;
+        commit<CTAS>(elected, tmemFullBar(a0));
+        if (a0) ++use1; else ++use0;
+        if (two) { commit<CTAS>(elected, tmemFullBar(1)); ++use1; }
+        ++accIt;
+        return true;
+      });
     }
   } else {
     // ---- epilogue: four warps for each accumulator ----
@@ -280,16 +345,14 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
     const uint32_t stagingWarp = stagingAll + uint32_t(warp - 2) * uint32_t(kStageTiles * kStageTileBytes);
     const uint32_t rowAddr = uint32_t(lane) * 128u, swz = uint32_t(lane & 7);
     uint32_t accIt = 0, uses = 0, tileCount = 0;
-    bool ok = true;
-    for (int it = pairIdx; it < p.items && ok; it += numPairs, ++accIt) {
-      const Item item = itemOf<ACCS>(p, it);
-      if (ACCS == 1 ? int(accIt & 1) != group : group >= item.count) continue;
-      int mIdx, nIdx;
-      tileCoord(p, item.tile, mIdx, nIdx);
-      const int row0 = ((mIdx * ACCS + item.first + (ACCS == 2 ? group : 0)) * CTAS + int(ctaRank)) * kBM + quarter * 32;
-      const int n0 = nIdx * p.bn, rowsValid = min(p.M - row0, 32);
+    forItems<CTAS, ACCS>(p, pairIdx, numPairs, [&](const Item& m) {
+      const uint32_t number = accIt++;
+      if (ACCS == 1 ? int(number & 1) != group : group >= m.count) return true;
+      const Group& g = p.g[m.group];
+      const int row0 = m.row + ((ACCS == 2 ? group : 0) * CTAS + int(ctaRank)) * kBM + quarter * 32;
+      const int n0 = m.col, rowsValid = min(g.M - row0, 32);
       // chunks of 32 accumulator columns that hold output
-      const int nChunks = rowsValid <= 0 ? 0 : (min(p.bn, p.N - n0) + 31) / 32;
+      const int nChunks = rowsValid <= 0 ? 0 : (min(p.bn, g.N - n0) + 31) / 32;
       uint4* saved = nullptr;                                           // of this warp's rows and the tile's first columns
       uint32_t z[24];
       if constexpr (EPI == kGate) { if (p.saved) saved = p.saved + (size_t(row0 / 32) * size_t(p.savedCols) + size_t(n0 / 32)) * (kSavedBlock / 16); }
@@ -297,9 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
         saved = p.saved + (size_t(row0 / 32) * size_t(p.savedCols) + size_t(n0 / 16)) * (kSavedBlock / 16);
         if (nChunks > 0) loadSaved(saved, lane, z);                     // on the way while the tile's last MMAs run
       }
-      ok = tc::mbarWait(tmemFullBar(group), uses & 1, abortWord, p.timeoutNs);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) { if (lane == 0) skinny::recordTimeout(p.status, 5, item.tile, group); break; }
+      if (!waitAll(tmemFullBar(group), uses & 1, abortWord, p.timeoutNs)) { if (lane == 0) skinny::recordTimeout(p.status, 5, m.tile, group); return false; }
       ++uses;
       tc::fenceAfterThreadSync();
       const uint32_t taddr = tmemBase + (uint32_t(quarter * 32) << 16) + uint32_t(group) * kAccStride;
@@ -315,11 +376,11 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
       auto drain = [&](uint32_t buf, int col) {                         // columns and rows past the output are clipped
         tc::fenceProxyAsyncShared();
         __syncwarp();
-        if (lane == 0) { tc::tmaStore2d(&maps.c, col, row0, buf); tc::bulkCommitGroup(); }
+        if (lane == 0) { tc::tmaStore2d(&g.c, col, row0, buf); tc::bulkCommitGroup(); }
       };
       if constexpr (EPI == kGateGrad) {
         // 32 columns of dh are 64 of dZ: [16 dG][16 dU][16 dG][16 dU], one staging tile
-        const int blocks = min(p.bn, p.N - n0) / 16;                    // saved blocks of this tile (N is a multiple of 16)
+        const int blocks = min(p.bn, g.N - n0) / 16;                    // saved blocks of this tile (N is a multiple of 16)
 #pragma unroll 1
         for (int c = 0; c < nChunks; ++c) {
           uint32_t r[32], o[16];
@@ -392,7 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
         if constexpr (CTAS == 2) tc::mbarArriveClusterTmem(leaderBars + 8u * uint32_t(2 * kMaxStages + 2 + group));
         else tc::mbarArrive(tmemEmptyBar(group));
       }
-    }
+      return true;
+    });
     if (lane == 0) tc::bulkWaitGroup<0>();
   }
 
@@ -408,8 +470,6 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
 // ------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------
-struct Operand { const void* ptr; int rows, cols; };    // as it lies in memory, row-major bf16
-
 struct Shape { int ctas, accs, bn; };
 
 struct Device { int sms = 0, index = -1; };
@@ -423,26 +483,43 @@ bool currentDevice(Device& d) {
   return d.sms > 0;
 }
 
-// The tile that is expected to take least. A k-block (64 of k) of a tile takes the longest of its MMAs (bn / 2 cycles per 16 of k and accumulator,
-// more where they all go into one accumulator) and its loads from L2 (about 56 bytes a cycle and SM); a tile adds its fill and its epilogue.
-Shape chooseShape(int M, int N, int K, int sms, int epi) {
+struct Sizes { int M, N, K; };
+int64_t tilesOf(const Sizes& z, const Shape& s) {
+  const int tileRows = kBM * s.ctas * s.accs;
+  return int64_t((z.M + tileRows - 1) / tileRows) * ((z.N + s.bn - 1) / s.bn);
+}
+// Expected cycles of a tile. A k-block (64 of k) takes the longest of its MMAs (bn / 2 cycles per 16 of k and accumulator, more where they
+// all go into one accumulator) and its loads from L2 (about 56 bytes a cycle and SM); a tile adds its epilogue, which with one
+// accumulator per tile hides under the next one's main loop.
+double tileCycles(const Sizes& z, const Shape& s, int epi) {
+  const double kBlocks = (z.K + kBK - 1) / kBK;
+  const double mma = 4.0 * s.accs * s.bn / 2 * (s.accs == 2 ? 1.0 : 1.36);
+  const double load = (s.accs * std::min(z.M, kBM) + s.bn / s.ctas) * 128.0 / 56;
+  const double epilogue = s.bn * (s.accs == 2 ? 16.0 : 8.0) * (epi == kStore ? 1.0 : 2.0), main = kBlocks * std::max(mma, load);
+  return s.accs == 2 ? main + 1500 + epilogue : std::max(main + 500, epilogue);
+}
+// The tile that is expected to take least.
+Shape chooseShape(const Sizes* z, int n, int sms, int epi) {
   Shape best{2, 2, 256};
   double least = 1e30;
-  const double kBlocks = (K + kBK - 1) / kBK;
   auto consider = [&](Shape s) {
-    const int tileRows = kBM * s.ctas * s.accs, units = sms / s.ctas;
-    const int64_t tiles = int64_t((M + tileRows - 1) / tileRows) * ((N + s.bn - 1) / s.bn);
-    double waves = double((tiles + units - 1) / units);
-    const int64_t rest = tiles % units;
-    if (s.accs == 2 && tiles > units && rest > 0 && 2 * rest <= units) waves -= 0.5;
-    const double rowsOfA = std::min(M, kBM);
-    const double mma = 4.0 * s.accs * s.bn / 2 * (s.accs == 2 ? 1.0 : 1.36);
-    const double load = (s.accs * rowsOfA + s.bn / s.ctas) * 128.0 / 56;
-    const double epilogue = s.bn * (s.accs == 2 ? 16.0 : 8.0) * (epi == kStore ? 1.0 : 2.0);
-    const double block = std::max(mma, load);
-    // with one accumulator per tile the epilogue hides under the next tile's main loop, but for the last one
-    const double cycles = s.accs == 2 ? waves * (kBlocks * block + 1500 + epilogue)
-                                      : waves * std::max(kBlocks * block + 500, epilogue) + 1500 + epilogue;
+    const int units = sms / s.ctas;
+    double cycles = 0, longest = 0;
+    if (n == 1) {
+      const int64_t tiles = tilesOf(z[0], s), rest = tiles % units;
+      double waves = double((tiles + units - 1) / units);
+      if (s.accs == 2 && tiles > units && rest > 0 && 2 * rest <= units) waves -= 0.5;
+      cycles = waves * tileCycles(z[0], s, epi);
+    } else {
+      double last = 0;
+      for (int i = 0; i < n; ++i) {
+        last = tileCycles(z[i], s, epi);
+        longest = std::max(longest, last);
+        cycles += double(tilesOf(z[i], s)) * last / units;
+      }
+      cycles = std::max(cycles + 0.5 * last, longest);
+    }
+    if (s.accs == 1) cycles += 1500 + s.bn * 8.0;
     if (cycles < least) { least = cycles; best = s; }
   };
   consider({2, 2, 256});
@@ -453,9 +530,45 @@ Shape chooseShape(int M, int N, int K, int sms, int epi) {
   return best;
 }
 
-template <bool A_MN, bool B_MN, int EPI, int CTAS, int ACCS>
-int launchAs(const Maps& maps, Params p, const Device& dev, cudaStream_t stream) {
-  auto kernel = ffnKernel<A_MN, B_MN, EPI, CTAS, ACCS>;
+// Shares the tiles of a launch out over its pairs: group by group, the longest tiles first; pairs that got one tile fewer than others take more
+// of the next group's. The last wave of all, if it fills at most half of the pairs, goes out as single accumulators.
+void shareOut(Params& p, int groups, const Shape& s, int units, int epi) {
+  int order[kMaxGroups] = {0, 1, 2};
+  double cost[kMaxGroups] = {};
+  for (int i = 0; i < groups; ++i) cost[i] = tileCycles(Sizes{p.g[i].M, p.g[i].N, p.g[i].K}, s, epi);
+  std::sort(order, order + groups, [&](int a, int b) { return cost[a] > cost[b]; });
+  int lateFirst = 0, late = 0;                // pairs [lateFirst, lateFirst + late), wrapping around, end `ahead` cycles after the others
+  double ahead = 0;
+  auto add = [&](int group, int start, int count, int first, int pairs, int halves) {
+    if (count > 0) p.seg[p.segments++] = Segment{group, start, count, first % units, pairs, halves};
+  };
+  p.segments = 0;
+  for (int i = 0; i < groups; ++i) {
+    const int group = order[i], tiles = p.g[group].tilesM * p.g[group].tilesN;
+    int done = 0;
+    if (late > 0) {
+      const int each = int(ahead / cost[group] + 0.5);
+      done = int(std::min<int64_t>(tiles, int64_t(each) * (units - late)));
+      add(group, 0, done, lateFirst + late, units - late, 0);
+    }
+    const int left = tiles - done, whole = left / units * units, rest = left - whole;
+    add(group, done, whole, lateFirst + late, units, 0);
+    if (rest) {
+      const bool halves = i == groups - 1 && s.accs == 2 && 2 * rest <= units && (whole || done || i > 0);
+      add(group, done + whole, rest, lateFirst + late, halves ? 2 * rest : rest, halves);
+      lateFirst = (lateFirst + late) % units; late = rest; ahead = cost[group];
+    } else if (done && done % (units - late)) {
+      const int some = done % (units - late);
+      lateFirst = (lateFirst + late) % units; late = some; ahead = cost[group];
+    } else if (left > 0 || done) {
+      late = 0;
+    }
+  }
+}
+
+template <bool B_MN, int EPI, int CTAS, int ACCS>
+int launchAs(Params& p, int groups, const Shape& s, const Device& dev, cudaStream_t stream) {
+  auto kernel = ffnKernel<B_MN, EPI, CTAS, ACCS>;
   // shared-memory opt-in and cluster occupancy belong to the device's copy of the kernel: resolved once per device
   static std::mutex mu;
   static int known[64] = {};
@@ -477,14 +590,16 @@ int launchAs(const Maps& maps, Params p, const Device& dev, cudaStream_t stream)
     }
     units = n;
   }
-  const int tiles = p.tilesM * p.tilesN;
-  units = std::min(units, tiles);
-  p.items = p.fullItems = tiles;
-  if (ACCS == 2) {
-    // a last wave that fills at most half of the pairs is issued as halves of tiles
-    const int rest = tiles % units;
-    if (tiles > units && rest > 0 && 2 * rest <= units) { p.fullItems = tiles - rest; p.items = p.fullItems + 2 * rest; }
+  int64_t tiles = 0;
+  for (int i = 0; i < groups; ++i) {
+    const Sizes z{p.g[i].M, p.g[i].N, p.g[i].K};
+    const int tileRows = kBM * CTAS * ACCS;
+    p.g[i].tilesM = (z.M + tileRows - 1) / tileRows; p.g[i].tilesN = (z.N + s.bn - 1) / s.bn;
+    if (tilesOf(z, s) > INT32_MAX / 4) { setError("feed-forward: the product is too large"); return 1; }
+    tiles += tilesOf(z, s);
   }
+  units = int(std::min<int64_t>(units, tiles));
+  shareOut(p, groups, s, units, EPI);
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = CTAS; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -492,38 +607,43 @@ int launchAs(const Maps& maps, Params p, const Device& dev, cudaStream_t stream)
   cfg.gridDim = dim3(unsigned(units * CTAS)); cfg.blockDim = dim3(kThreads); cfg.stream = stream;
   cfg.dynamicSmemBytes = size_t(p.stages) * size_t(ACCS * p.aBytes + p.bn / CTAS * kBK * 2) + kStagingBytes + kBarrierBytes + 1024;
   cfg.attrs = attr; cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   if (e != cudaSuccess) { setError(std::string("feed-forward launch: ") + cudaGetErrorString(e)); return 1; }
   return 0;
 }
 
-// C[M, N] (or the gated forms) = sum over k; an operand is [rows of D, K] row-major, or [K, rows of D] where its _MN is set
-template <bool A_MN, bool B_MN, int EPI>
-int product(const void* A, const void* B, void* C, int M, int N, int K, void* saved, int activation, uint32_t* status, cudaStream_t stream) {
+// C[M, N] (or the gated forms) = sum over k of A(m, k) B(n, k). A is [M, K] row-major, or [K, M] with aMn; B is [N, K], or [K, N] with B_MN.
+struct Product { const void *A, *B; void* C; int M, N, K; bool aMn; };
+template <bool B_MN, int EPI>
+int run(const Product* products, int n, void* saved, int activation, uint32_t* status, cudaStream_t stream) {
   Device dev;
   if (!currentDevice(dev)) return 1;
-  const Shape s = chooseShape(M, N, K, dev.sms, EPI);
   Params p{};
-  p.M = M; p.N = N; p.K = K; p.bn = s.bn;
-  const int tileRows = kBM * s.ctas * s.accs;
-  p.tilesM = (M + tileRows - 1) / tileRows; p.tilesN = (N + s.bn - 1) / s.bn;
-  // Few rows of A (as many as one tile has at most) take only their own room in a stage: the MMA's other rows read what lies behind, and
-  // rows of the accumulator that are no rows of D are never stored.
-  const int boxRows = A_MN || s.ctas == 2 ? kBM : std::min(kBM, (M + 7) / 8 * 8);
-  p.aBytes = boxRows * kBK * 2;
-  const int stageBytes = s.accs * p.aBytes + s.bn / s.ctas * kBK * 2;
-  p.stages = std::min((kSmemLimit - kBarrierBytes - 1024 - kStagingBytes) / stageBytes, kMaxStages);
-  const int outCols = EPI == kGate ? N / 2 : EPI == kGateGrad ? 2 * N : N;
-  p.C = static_cast<__nv_bfloat16*>(C); p.ldc = outCols;
-  p.saved = static_cast<uint4*>(saved); p.savedCols = EPI == kGate ? N / 32 : N / 16;
+  Sizes z[kMaxGroups] = {};
+  for (int i = 0; i < n; ++i) z[i] = Sizes{products[i].M, products[i].N, products[i].K};
+  const Shape s = chooseShape(z, n, dev.sms, EPI);
+  p.bn = s.bn;
+  p.saved = static_cast<uint4*>(saved); p.savedCols = EPI == kGate ? z[0].N / 32 : z[0].N / 16;
   p.activation = activation; p.status = status; p.timeoutNs = 2ull * 1000 * 1000 * 1000;
-  Maps maps{};
   auto bf16Map = [](CUtensorMap& m, const void* ptr, int rows, int cols, int boxRows) {
     return makeTensorMap(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ptr, uint64_t(rows), uint64_t(cols) * 2, uint64_t(cols) * 2, uint32_t(boxRows));
   };
-  if (!(A_MN ? bf16Map(maps.a, A, K, M, kBK) : bf16Map(maps.a, A, M, K, boxRows)) ||
-      !(B_MN ? bf16Map(maps.b, B, K, N, kBK) : bf16Map(maps.b, B, N, K, s.bn / s.ctas)) || !bf16Map(maps.c, C, M, outCols, 32)) return 1;
-  return s.ctas == 2 ? launchAs<A_MN, B_MN, EPI, 2, 2>(maps, p, dev, stream) : launchAs<A_MN, B_MN, EPI, 1, 1>(maps, p, dev, stream);
+  for (int i = 0; i < n; ++i) {
+    const Product& q = products[i];
+    Group& g = p.g[i];
+    g.M = q.M; g.N = q.N; g.K = q.K; g.aMn = q.aMn;
+    // Few rows of A take only their own room in a stage: the MMA's other rows read what lies behind, and rows of the accumulator that are no
+    // rows of the result are never stored.
+    const int boxRows = q.aMn || s.ctas == 2 ? kBM : std::min(kBM, (q.M + 7) / 8 * 8);
+    g.aBytes = boxRows * kBK * 2;
+    p.aBytes = std::max(p.aBytes, g.aBytes);
+    const int outCols = EPI == kGate ? q.N / 2 : EPI == kGateGrad ? 2 * q.N : q.N;
+    if (!(q.aMn ? bf16Map(g.a, q.A, q.K, q.M, kBK) : bf16Map(g.a, q.A, q.M, q.K, boxRows)) ||
+        !(B_MN ? bf16Map(g.b, q.B, q.K, q.N, kBK) : bf16Map(g.b, q.B, q.N, q.K, s.bn / s.ctas)) || !bf16Map(g.c, q.C, q.M, outCols, 32)) return 1;
+  }
+  const int stageBytes = s.accs * p.aBytes + s.bn / s.ctas * kBK * 2;
+  p.stages = std::min((kSmemLimit - kBarrierBytes - 1024 - kStagingBytes) / stageBytes, kMaxStages);
+  return s.ctas == 2 ? launchAs<B_MN, EPI, 2, 2>(p, n, s, dev, stream) : launchAs<B_MN, EPI, 1, 1>(p, n, s, dev, stream);
 }
 
 bool sizesFit(int tokens, int hidden, int intermediate, int activation) {
@@ -548,9 +668,10 @@ int purlin_ffn_forward(const void* x, const void* wGateUp, const void* wDown, vo
   NvtxRange range("ffnForward", size_t(tokens) * size_t(hidden) * 2);
   if (!sizesFit(tokens, hidden, intermediate, activation)) return 1;
   if (reinterpret_cast<uintptr_t>(saved) % 16) { setError("feed-forward: the saved pre-activations need 16-byte alignment"); return 1; }
+  const Product up{x, wGateUp, hOut, tokens, 2 * intermediate, hidden, false};
   const int rc = !saved && activation == PURLIN_ACT_SILU
       ? purlin_gemm_bf16(x, wGateUp, hOut, tokens, 2 * intermediate, hidden, PURLIN_EPI_SWIGLU, 0, status, stream)
-      : product<false, false, kGate>(x, wGateUp, hOut, tokens, 2 * intermediate, hidden, saved, activation, status, static_cast<cudaStream_t>(stream));
+      : run<false, kGate>(&up, 1, saved, activation, status, static_cast<cudaStream_t>(stream));
   if (rc || !y) return rc;
   return purlin_gemm_bf16(hOut, wDown, y, tokens, hidden, intermediate, PURLIN_EPI_STORE, 0, status, stream);
 }
@@ -561,13 +682,16 @@ int purlin_ffn_backward(const void* x, const void* wGateUp, const void* wDown, c
   if (!sizesFit(tokens, hidden, intermediate, activation)) return 1;
   if (reinterpret_cast<uintptr_t>(saved) % 16) { setError("feed-forward: the saved pre-activations need 16-byte alignment"); return 1; }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int rc = 0;
-  if (dx || dGateUp)
-    rc = product<false, true, kGateGrad>(dy, wDown, dz, tokens, intermediate, hidden, const_cast<void*>(saved), activation, status, s);
-  if (!rc && dx) rc = product<false, true, kStore>(dz, wGateUp, dx, tokens, hidden, 2 * intermediate, nullptr, activation, status, s);
-  if (!rc && dGateUp) rc = product<true, true, kStore>(dz, x, dGateUp, 2 * intermediate, hidden, tokens, nullptr, activation, status, s);
-  if (!rc && dDown) rc = product<true, true, kStore>(dy, h, dDown, hidden, intermediate, tokens, nullptr, activation, status, s);
-  return rc;
+  if (dx || dGateUp) {
+    const Product gradZ{dy, wDown, dz, tokens, intermediate, hidden, false};
+    if (run<true, kGateGrad>(&gradZ, 1, const_cast<void*>(saved), activation, status, s)) return 1;
+  }
+  Product grads[kMaxGroups];
+  int n = 0;
+  if (dx) grads[n++] = Product{dz, wGateUp, dx, tokens, hidden, 2 * intermediate, false};
+  if (dGateUp) grads[n++] = Product{dz, x, dGateUp, 2 * intermediate, hidden, tokens, true};
+  if (dDown) grads[n++] = Product{dy, h, dDown, hidden, intermediate, tokens, true};
+  return n ? run<true, kStore>(grads, n, nullptr, activation, status, s) : 0;
 }
 
 }  // extern "C"

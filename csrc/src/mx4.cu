@@ -33,8 +33,11 @@ constexpr int kScaleRows = 128, kScaleCols = 128, kScaleBytes = 512;
 // ------------------------------------------------------------------------------------------
 // quantisation and the way back: bound by memory
 // ------------------------------------------------------------------------------------------
-// A thread has 8 neighbouring values, four threads a block, sixteen a word of the scales; a warp 256 columns of one row per step.
-constexpr int kVec = 8, kWarpCols = 32 * kVec, kQuantThreads = 256, kUnroll = 4;
+// Four lanes have the 32 values of a block (8 each, 16 bytes of bf16 or fp16), a warp 256 columns, and a step of a warp is four of those side by
+// side in one row. The scale needs the exponent of the largest magnitude only, a byte, so the four blocks of a lane travel through the
+// shuffles in one word, and four more shuffles' worth of bytes become the words of the scales' layout in two. With one shuffle chain per block and
+// 64-bit index arithmetic the instructions, not the memory, were the bound (8192 x 8192 there and back 104 us).
+constexpr int kVec = 8, kWarpCols = 32 * kVec, kQuantThreads = 256, kUnroll = 4, kStepCols = kUnroll * kWarpCols;
 
 PURLIN_D uint4 ldOnce(const void* p) {
   uint4 v;
@@ -48,6 +51,20 @@ template <int TYPE> PURLIN_D Raw<TYPE> loadRaw(const unsigned char* p) {
   r.v[0] = ldOnce(p);
   if constexpr (TYPE == PURLIN_MX4_FP32) r.v[1] = ldOnce(p + 16);
   return r;
+}
+// The exponent field that the largest magnitude has in fp32: 255 for infinities and NaNs, 0 for zeros (and below 2^-126, which the scale does not tell
+// apart). Magnitudes compare as their bit patterns.
+template <int TYPE> PURLIN_D uint32_t peakExponent(const Raw<TYPE>& r) {
+  if constexpr (TYPE == PURLIN_MX4_FP32) {
+    uint32_t m = max(max(r.v[0].x & 0x7fffffffu, r.v[0].y & 0x7fffffffu), max(r.v[0].z & 0x7fffffffu, r.v[0].w & 0x7fffffffu));
+    m = max(m, max(max(r.v[1].x & 0x7fffffffu, r.v[1].y & 0x7fffffffu), max(r.v[1].z & 0x7fffffffu, r.v[1].w & 0x7fffffffu)));
+    return m >> 23;
+  } else {
+    const uint32_t m = __vmaxu2(__vmaxu2(r.v[0].x & 0x7fff7fffu, r.v[0].y & 0x7fff7fffu), __vmaxu2(r.v[0].z & 0x7fff7fffu, r.v[0].w & 0x7fff7fffu));
+    const uint32_t top = max(m & 0xffffu, m >> 16);
+    if constexpr (TYPE == PURLIN_MX4_BF16) return top >> 7;
+    else return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(top)))) >> 23;
+  }
 }
 template <int TYPE> PURLIN_D void toFloats(const Raw<TYPE>& r, float (&f)[kVec]) {
   const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
@@ -71,54 +88,55 @@ PURLIN_D size_t scaleOffset(int row, int col, int colBlocks) {       // of the s
   return (size_t(row / kScaleRows) * size_t(colBlocks) + size_t(col / kScaleCols)) * kScaleBytes + size_t(row % 32) * 16 + size_t(row / 32 % 4) * 4 + size_t(col / kBlock % 4);
 }
 
-// One step of a warp: 256 columns of a row. Rows past the last one (up to the scales' 128) write their zeros.
+// Rows past the last one (up to the scales' 128) write their zeros.
 template <int TYPE>
 __global__ void __launch_bounds__(kQuantThreads) quantizeKernel(const unsigned char* __restrict__ x, unsigned char* __restrict__ data, unsigned char* __restrict__ scales,
-                                                                int rows, int cols, int steps, int64_t total) {
+                                                                int rows, int cols, uint32_t steps, uint32_t total) {
   tc::gridDependencyWait();
   tc::gridLaunchDependents();
   constexpr int kSize = TYPE == PURLIN_MX4_FP32 ? 4 : 2;
   const int lane = threadIdx.x & 31;
-  const int64_t warp = int64_t(blockIdx.x) * (kQuantThreads / 32) + (threadIdx.x >> 5), warps = int64_t(gridDim.x) * (kQuantThreads / 32);
+  const uint32_t warps = gridDim.x * (kQuantThreads / 32);
   const int colBlocks = (cols + kScaleCols - 1) / kScaleCols;
-  for (int64_t i0 = warp; i0 < total; i0 += warps * kUnroll) {
+  for (uint32_t i = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); i < total; i += warps) {
+    const int row = int(i / steps), col = int(i % steps) * kStepCols + lane * kVec;
+    const size_t at = size_t(row) * size_t(cols) + size_t(col);
     Raw<TYPE> raw[kUnroll];
-    int row[kUnroll], col[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int64_t i = i0 + u * warps;
-      row[u] = i < total ? int(i / steps) : INT32_MAX;
-      col[u] = int(i % steps) * kWarpCols + lane * kVec;
       raw[u].v[0] = make_uint4(0, 0, 0, 0);
       if constexpr (TYPE == PURLIN_MX4_FP32) raw[u].v[1] = make_uint4(0, 0, 0, 0);
-      if (row[u] < rows && col[u] < cols) raw[u] = loadRaw<TYPE>(x + (size_t(row[u]) * size_t(cols) + size_t(col[u])) * kSize);
+      if (row < rows && col + u * kWarpCols < cols) raw[u] = loadRaw<TYPE>(x + (at + size_t(u * kWarpCols)) * kSize);
     }
+    uint32_t peaks = 0;                                       // a byte for each of the four blocks
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) peaks |= peakExponent<TYPE>(raw[u]) << (8 * u);
+    peaks = __vmaxu4(peaks, __shfl_xor_sync(0xffffffffu, peaks, 1));
+    peaks = __vmaxu4(peaks, __shfl_xor_sync(0xffffffffu, peaks, 2));
+    // a scale is the exponent less 2, at least 0, and stays 255
+    const uint32_t bad = __vcmpeq4(peaks, 0xffffffffu), scale4 = __vsubus4(peaks, 0x02020202u) | bad;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
+      const uint32_t scale = scale4 >> (8 * u) & 255u;
+      const float inverse = __uint_as_float((254u - scale) << 23);       // (of a scale of 255 not used)
       float f[kVec];
       toFloats<TYPE>(raw[u], f);
-      uint32_t peak = 0;                                    // magnitudes as bit patterns: a NaN is above an infinity, which is above all others
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) peak = max(peak, __float_as_uint(f[e]) & 0x7fffffffu);
-      peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
-      peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
-      const bool finite = peak < 0x7f800000u;
-      const int scale = finite ? max(int(peak >> 23) - 2, 0) : 255;
-      const float inverse = finite ? __uint_as_float(uint32_t(254 - scale) << 23) : 0.f;
       uint32_t codes = 0;
 #pragma unroll
-      for (int e = 0; e < kVec; e += 2) {
-        const float2 v = finite ? make_float2(f[e] * inverse, f[e + 1] * inverse) : make_float2(0.f, 0.f);
-        codes |= uint32_t(__nv_cvt_float2_to_fp4x2(v, __NV_E2M1, cudaRoundNearest)) << (4 * e);
-      }
-      // four blocks' scales meet in the first of their sixteen threads
-      uint32_t word = uint32_t(scale) << (8 * (lane / 4 % 4));
-      word |= __shfl_xor_sync(0xffffffffu, word, 4);
-      word |= __shfl_xor_sync(0xffffffffu, word, 8);
-      if (row[u] == INT32_MAX || col[u] >= colBlocks * kScaleCols) continue;
-      if (row[u] < rows && col[u] < cols) *reinterpret_cast<uint32_t*>(data + (size_t(row[u]) * size_t(cols) + size_t(col[u])) / 2) = codes;
-      if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(scales + scaleOffset(row[u], col[u], colBlocks)) = word;
+      for (int e = 0; e < kVec; e += 2)
+        codes |= uint32_t(__nv_cvt_float2_to_fp4x2(make_float2(f[e] * inverse, f[e + 1] * inverse), __NV_E2M1, cudaRoundNearest)) << (4 * e);
+      if (scale == 255u) codes = 0;
+      if (row < rows && col + u * kWarpCols < cols) *reinterpret_cast<uint32_t*>(data + (at + size_t(u * kWarpCols)) / 2) = codes;
     }
+    // Four blocks side by side (lanes 0, 4, 8, 12 of sixteen) make a word of the scales, and each lane has a byte for each of four such words:
+    // a transposition of 4 x 4 bytes, after which the q-th four lanes hold the word of step q.
+    const int q = lane / 4 % 4;
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, scale4, 4);
+    const uint32_t pair = q & 1 ? __byte_perm(other, scale4, 0x7351) : __byte_perm(scale4, other, 0x6240);    // [word q%2: two blocks][word q%2 + 2: two blocks]
+    const uint32_t far = __shfl_xor_sync(0xffffffffu, pair, 8);
+    const uint32_t word = q & 2 ? __byte_perm(far, pair, 0x7632) : __byte_perm(pair, far, 0x5410);
+    const int first = int(i % steps) * kStepCols + q * kWarpCols + lane / 16 * kScaleCols;
+    if (lane % 4 == 0 && first < cols) *reinterpret_cast<uint32_t*>(scales + scaleOffset(row, first, colBlocks)) = word;
   }
 }
 
@@ -128,28 +146,28 @@ PURLIN_D float powerOf(uint32_t scale) {      // 2^(scale - 127); 2^-127 is belo
 
 template <int TYPE>
 __global__ void __launch_bounds__(kQuantThreads) dequantizeKernel(const unsigned char* __restrict__ data, const unsigned char* __restrict__ scales, unsigned char* __restrict__ out,
-                                                                  int rows, int cols, int steps, int64_t total) {
+                                                                  int rows, int cols, uint32_t steps, uint32_t total) {
   tc::gridDependencyWait();
   tc::gridLaunchDependents();
   const int lane = threadIdx.x & 31;
-  const int64_t warp = int64_t(blockIdx.x) * (kQuantThreads / 32) + (threadIdx.x >> 5), warps = int64_t(gridDim.x) * (kQuantThreads / 32);
+  const uint32_t warps = gridDim.x * (kQuantThreads / 32);
   const int colBlocks = (cols + kScaleCols - 1) / kScaleCols;
-  for (int64_t i0 = warp; i0 < total; i0 += warps * kUnroll) {
+  for (uint32_t i = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); i < total; i += warps) {
+    const int row = int(i / steps), col = int(i % steps) * kStepCols + lane * kVec;
+    const size_t at = size_t(row) * size_t(cols) + size_t(col);
+    const unsigned char* scaleAt = scales + scaleOffset(row, col, colBlocks);          // (256 columns further on: two blocks of 512 bytes)
     uint32_t codes[kUnroll], scale[kUnroll];
-    int64_t at[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int64_t i = i0 + u * warps;
-      const int row = int(i / steps), col = int(i % steps) * kWarpCols + lane * kVec;
-      at[u] = i < total && col < cols ? int64_t(row) * cols + col : -1;
-      if (at[u] >= 0) {
-        codes[u] = *reinterpret_cast<const uint32_t*>(data + at[u] / 2);
-        scale[u] = scales[scaleOffset(row, col, colBlocks)];
+      codes[u] = scale[u] = 0;
+      if (col + u * kWarpCols < cols) {
+        codes[u] = *reinterpret_cast<const uint32_t*>(data + (at + size_t(u * kWarpCols)) / 2);
+        scale[u] = scaleAt[u * (kWarpCols / kScaleCols * kScaleBytes)];
       }
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      if (at[u] < 0) continue;
+      if (col + u * kWarpCols >= cols) continue;
       const float power = powerOf(scale[u]);
       float f[kVec];
 #pragma unroll
@@ -160,11 +178,11 @@ __global__ void __launch_bounds__(kQuantThreads) dequantizeKernel(const unsigned
         f[e + 1] = v.y * power;
       }
       if constexpr (TYPE == PURLIN_MX4_FP32) {
-        float4* to = reinterpret_cast<float4*>(out + at[u] * 4);
+        float4* to = reinterpret_cast<float4*>(out + (at + size_t(u * kWarpCols)) * 4);
         to[0] = make_float4(f[0], f[1], f[2], f[3]);
         to[1] = make_float4(f[4], f[5], f[6], f[7]);
       } else {
-        *reinterpret_cast<uint4*>(out + at[u] * 2) = make_uint4(skinny::pack2(f[0], f[1]), skinny::pack2(f[2], f[3]), skinny::pack2(f[4], f[5]), skinny::pack2(f[6], f[7]));
+        *reinterpret_cast<uint4*>(out + (at + size_t(u * kWarpCols)) * 2) = make_uint4(skinny::pack2(f[0], f[1]), skinny::pack2(f[2], f[3]), skinny::pack2(f[4], f[5]), skinny::pack2(f[6], f[7]));
       }
     }
   }
@@ -616,17 +634,26 @@ bool launched(cudaError_t e) {
 bool sizesFit(int rows, int cols) {
   if (rows <= 0 || cols <= 0) { setError("mx4: dimensions must be positive"); return false; }
   if (cols % kBlock) { setError("mx4: the columns must be a multiple of 32"); return false; }
-  if (rows > INT32_MAX - kScaleRows || cols > INT32_MAX - kWarpCols) { setError("mx4: dimensions too large"); return false; }
+  if (rows > INT32_MAX - kScaleRows || cols > INT32_MAX - kStepCols) { setError("mx4: dimensions too large"); return false; }
+  return true;
+}
+
+// steps of a row and of all rows, their number rounded up to a multiple of `unit`
+bool stepsOf(int rows, int cols, int unit, uint32_t& steps, uint32_t& total) {
+  steps = uint32_t((cols + kStepCols - 1) / kStepCols);
+  const uint64_t all = uint64_t((rows + unit - 1) / unit) * uint64_t(unit) * steps;
+  if (all > uint64_t(INT32_MAX)) { setError("mx4: the tensor is too large"); return false; }      // the walk counts in 32 bits
+  total = uint32_t(all);
   return true;
 }
 
 template <typename... A>
-int launchRows(void (*kernel)(A...), int64_t total, const Device& dev, cudaStream_t stream, A... args) {
+int launchRows(void (*kernel)(A...), uint32_t total, const Device& dev, cudaStream_t stream, A... args) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
   constexpr int kWarps = kQuantThreads / 32;
-  cfg.gridDim = dim3(unsigned(std::min<int64_t>((total + kWarps - 1) / kWarps, int64_t(dev.sms) * 8)));
+  cfg.gridDim = dim3(std::min((total + kWarps - 1) / kWarps, uint32_t(dev.sms) * 8u));
   cfg.blockDim = dim3(kQuantThreads); cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 1;
   return launched(cudaLaunchKernelEx(&cfg, kernel, args...)) ? 0 : 1;
 }
@@ -763,8 +790,8 @@ int purlin_mx4_quantize(const void* x, int dtype, void* data, void* scales, int 
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales)) % 16) { setError("mx4: tensors must start on a 16-byte boundary"); return 1; }
   Device dev;
   if (!currentDevice(dev)) return 1;
-  const int steps = (cols + kWarpCols - 1) / kWarpCols;
-  const int64_t total = int64_t((rows + kScaleRows - 1) / kScaleRows * kScaleRows) * steps;
+  uint32_t steps, total;
+  if (!stepsOf(rows, cols, kScaleRows, steps, total)) return 1;
   auto kernel = dtype == PURLIN_MX4_BF16 ? quantizeKernel<PURLIN_MX4_BF16> : dtype == PURLIN_MX4_FP16 ? quantizeKernel<PURLIN_MX4_FP16>
               : dtype == PURLIN_MX4_FP32 ? quantizeKernel<PURLIN_MX4_FP32> : nullptr;
   if (!kernel) { setError("mx4: unknown type"); return 1; }
@@ -778,8 +805,8 @@ int purlin_mx4_dequantize(const void* data, const void* scales, void* out, int d
   if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales)) % 16) { setError("mx4: tensors must start on a 16-byte boundary"); return 1; }
   Device dev;
   if (!currentDevice(dev)) return 1;
-  const int steps = (cols + kWarpCols - 1) / kWarpCols;
-  const int64_t total = int64_t(rows) * steps;
+  uint32_t steps, total;
+  if (!stepsOf(rows, cols, 1, steps, total)) return 1;
   auto kernel = dtype == PURLIN_MX4_BF16 ? dequantizeKernel<PURLIN_MX4_BF16> : dtype == PURLIN_MX4_FP32 ? dequantizeKernel<PURLIN_MX4_FP32> : nullptr;
   if (!kernel) { setError("mx4: values come back in bf16 or fp32"); return 1; }
   return launchRows(kernel, total, dev, static_cast<cudaStream_t>(stream), static_cast<const unsigned char*>(data), static_cast<const unsigned char*>(scales),

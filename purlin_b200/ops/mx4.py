@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes as C
 from contextlib import nullcontext
-from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
 import torch
@@ -44,24 +43,29 @@ def scale_bytes(rows: int, cols: int) -> int:
     return -(-rows // 128) * -(-cols // 128) * 512
 
 
-@dataclass(frozen=True)
 class Mx4Tensor:
     """A [rows, cols] tensor in 4-bit microscaled form. ``data``: uint8 [rows, cols / 2], the even column in a byte's low half. ``scales``: uint8, a
     byte b per 32 columns of a row for 2^(b - 127) (255: the block stands for NaNs), in the tensor cores' order: blocks of 512 bytes for
     128 rows x 128 columns, [rows / 128][cols / 128][row % 32][row / 32 % 4][col / 32 % 4], zeros past the edges."""
-    data: torch.Tensor
-    scales: torch.Tensor
+    __slots__ = ("data", "scales")
 
-    def __post_init__(self):
-        d, s = self.data, self.scales
-        if d.dtype != torch.uint8 or s.dtype != torch.uint8:
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor):
+        if data.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError("data and scales are uint8 tensors")
-        if d.dim() != 2 or d.shape[1] == 0 or d.shape[1] % 16 or s.numel() != scale_bytes(d.shape[0], 2 * d.shape[1]):
+        if data.dim() != 2 or data.shape[1] == 0 or data.shape[1] % 16 or scales.numel() != scale_bytes(data.shape[0], 2 * data.shape[1]):
             raise ValueError("data is [rows, cols / 2] with cols a multiple of 32, and scales has 512 bytes for every 128 rows x 128 columns")
-        if not (d.is_cuda and s.device == d.device and d.is_contiguous() and s.is_contiguous()):
+        if not (data.is_cuda and scales.device == data.device and data.is_contiguous() and scales.is_contiguous()):
             raise ValueError("data and scales must be contiguous CUDA tensors on one device")
-        if (d.data_ptr() | s.data_ptr()) % 16:
+        if (data.data_ptr() | scales.data_ptr()) % 16:
             raise ValueError("data and scales must start on a 16-byte boundary")
+        self.data, self.scales = data, scales
+
+    @classmethod
+    def _empty(cls, rows: int, cols: int, device) -> "Mx4Tensor":
+        q = cls.__new__(cls)                 # (what it is made of needs no check)
+        q.data = torch.empty((rows, cols // 2), dtype=torch.uint8, device=device)
+        q.scales = torch.empty(scale_bytes(rows, cols), dtype=torch.uint8, device=device)
+        return q
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -105,18 +109,13 @@ def _rows(x: torch.Tensor) -> int:
     return x.numel() // x.shape[-1]
 
 
-def _empty(rows: int, cols: int, device) -> Mx4Tensor:
-    both = torch.empty(rows * cols // 2 + scale_bytes(rows, cols), dtype=torch.uint8, device=device)     # (a row is a multiple of 16 bytes)
-    return Mx4Tensor(both[:rows * cols // 2].view(rows, cols // 2), both[rows * cols // 2:])
-
-
 def quantize_mx4(x: torch.Tensor) -> Mx4Tensor:
     """``x [..., cols]`` (bf16, fp16 or fp32, contiguous, cols a multiple of 32) as an ``Mx4Tensor`` of its rows. A block's power of two is that of its
     largest magnitude over 4, at least 2^-127; values are rounded to the nearest of the format, ties to the even code, and above 6 times the power
     to 6. A block that holds an infinity or a NaN stands for NaNs."""
     _check_dense(x)
     rows, cols = _rows(x), x.shape[-1]
-    q = _empty(rows, cols, x.device)
+    q = Mx4Tensor._empty(rows, cols, x.device)
     if rows:
         lib = _lib()
         with _on(x.device):

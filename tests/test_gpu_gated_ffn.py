@@ -76,7 +76,7 @@ def test_outputs_and_gradients_against_64_bits(t, h, i, activation):
         assert (err <= tol).all(), f"{name}: {(err / tol).max().item()} of what rounding allows"
 
 
-@pytest.mark.parametrize("t,h,i", [(40, 2048, 1024), (513, 2048, 4096), (2100, 4096, 1024)])
+@pytest.mark.parametrize("t,h,i", [(40, 2048, 1024), (513, 2048, 4096), (2100, 4096, 1024), (4099, 2048, 2048), (9000, 1024, 4096)])
 def test_gradients_on_small_integers_are_the_products(t, h, i):
     # Every product of the block, in every order of its operands, exact: with a gate of 128 the sigmoid is 1 (act = g, act' = 1), all values
     # are small whole numbers that bf16 holds, and all sums are exact in fp32.
