@@ -255,13 +255,13 @@ PURLIN_D void loadScalesHere(uint32_t smemDst, const CUtensorMap* map, int y, in
 
 // ---- many rows: 256 rows of A x up to 256 rows of W per CTA pair ----
 // One accumulator of 256 columns; the scales of a stage take the columns behind it (two sets in turn). The epilogue gives the accumulator back
-// as soon as its values are in registers, activated and packed, and stores them under the next main loop.
-constexpr int kWideThreads = 32 * 10, kWideStages = 5, kMaxCols = 256;
+// as soon as its values are in registers; it activates, packs and stores them under the next main loop.
+constexpr int kWideThreads = 32 * 10, kWideStages = 6, kMaxCols = 256;      // (4 stages were 5 % slower, 5 by 1 to 2 %)
 constexpr int kWideStage = kABytes + kMaxCols / 2 * 128 + 3 * kScaleStage;      // [A][B half][scales A][scales B: two blocks of rows]
-constexpr int kStageTileBytes = 32 * 128, kWideStaging = 8 * kStageTileBytes;
+constexpr int kStageTileBytes = 32 * 64, kWideStaging = 8 * kStageTileBytes;      // 32 rows x 32 columns of the output per epilogue warp
 constexpr int kBarrierBytes = 256;
 constexpr int kScaleTmem = 256, kScaleSet = 32;                                   // columns: [A k-block 0, 1: 4 each][B k-block 0, 1: 8 each]
-constexpr size_t kWideSmem = 1024 + size_t(kWideStages) * kWideStage + kWideStaging + kBarrierBytes;
+constexpr size_t kWideSmem = size_t(kWideStages) * kWideStage + kWideStaging + kBarrierBytes;
 static_assert(kWideSmem <= size_t(kSmemLimit) && kWideStage % 1024 == 0, "the ring and the staging tiles fit one CTA per SM");
 
 struct WideParams {
@@ -285,10 +285,8 @@ PURLIN_D WideItem wideItem(const WideParams& p, int it) {
 
 template <bool SWIGLU>
 __global__ void __launch_bounds__(kWideThreads, 1) mx4WideKernel(const __grid_constant__ Maps maps, const __grid_constant__ WideParams p) {
-  extern __shared__ unsigned char smemRaw[];
-  const uint32_t rawAddr = tc::smemAddr(smemRaw);
-  const uint32_t base = (rawAddr + 1023u) & ~1023u;
-  unsigned char* smem = smemRaw + (base - rawAddr);
+  extern __shared__ __align__(1024) unsigned char smem[];     // swizzled tiles need 1024-byte alignment
+  const uint32_t base = tc::smemAddr(smem);
   const uint32_t stagingAll = base + uint32_t(kWideStages) * kWideStage, barBase = stagingAll + kWideStaging;
   auto fullBar = [&](uint32_t s) { return barBase + 8u * s; };
   auto emptyBar = [&](uint32_t s) { return barBase + 8u * (uint32_t(kWideStages) + s); };
@@ -384,7 +382,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4WideKernel(const __grid_co
     }
   } else {
     // ---- epilogue: two warps per quarter of the lanes, each up to two units of 64 accumulator columns ----
-    constexpr int kOutWords = SWIGLU ? 16 : 32;        // packed outputs of a unit
+    constexpr int kOutWords = SWIGLU ? 8 : 16;         // packed outputs of 32 accumulator columns
     const int quarter = warp & 3, half = (warp - 2) / 4;
     const uint32_t buf = stagingAll + uint32_t(warp - 2) * kStageTileBytes;
     uint32_t use = 0;
@@ -398,44 +396,46 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4WideKernel(const __grid_co
       if (!ok) { if (lane == 0) skinny::recordTimeout(p.status, 5, it, 0); break; }
       tc::fenceAfterThreadSync();
       const uint32_t taddr = tmemBase + (uint32_t(quarter * 32) << 16) + uint32_t(first * 64);
-      uint32_t o[2][kOutWords];
+      // all of this warp's values first: the accumulator goes back before any of them is activated, packed or stored
+      uint32_t r[4][32];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (u < count) {
+      for (int c = 0; c < 4; ++c)
+        if (c < 2 * count) tc::tmemLoad32(taddr + uint32_t(c * 32), r[c]);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t r[32];
-            tc::tmemLoad32(taddr + uint32_t(u * 64 + c * 32), r);
-            tc::tmemLoadWaitFor(r);
-            if constexpr (SWIGLU) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                o[u][c * 8 + i] = skinny::pack2(skinny::siluOf(__uint_as_float(r[2 * i])) * __uint_as_float(r[16 + 2 * i]),
-                                                skinny::siluOf(__uint_as_float(r[2 * i + 1])) * __uint_as_float(r[17 + 2 * i]));
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[u][c * 16 + i] = skinny::pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-            }
-          }
-        }
-      }
+      for (int c = 0; c < 4; ++c)
+        if (c < 2 * count) tc::tmemLoadWaitFor(r[c]);
       tc::fenceBeforeThreadSync();
       __syncwarp();
       if (lane == 0) tc::mbarArriveClusterTmem(leaderBars + 8u * (2 * kWideStages + 1));
-      // staging: 32 rows of 128 bytes (64 columns), or of 64 bytes (32 columns) with the gate, swizzled as the store's map says
+      // Staging: 32 rows of 64 bytes (32 columns) with the 64-byte swizzle. Without the gate that is 32 accumulator columns, with it 64.
+      constexpr int kChunks = SWIGLU ? 2 : 1;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (u < count) {
+      for (int u = 0; u < 4 / kChunks; ++u) {
+        if (u * kChunks < 2 * count) {
           if (lane == 0) tc::bulkWaitGroupRead<0>();
           __syncwarp();
 #pragma unroll
-          for (int j = 0; j < kOutWords / 4; ++j) {
-            const uint32_t at = SWIGLU ? uint32_t(lane) * 64u + (uint32_t(j) ^ uint32_t(lane >> 1 & 3)) * 16u : uint32_t(lane) * 128u + (uint32_t(j) ^ uint32_t(lane & 7)) * 16u;
-            tc::stShared16(buf + at, o[u][4 * j], o[u][4 * j + 1], o[u][4 * j + 2], o[u][4 * j + 3]);
+          for (int c = 0; c < kChunks; ++c) {
+            const uint32_t (&v)[32] = r[kChunks * u + c];
+            uint32_t o[kOutWords];
+            if constexpr (SWIGLU) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                o[i] = skinny::pack2(skinny::siluOf(__uint_as_float(v[2 * i])) * __uint_as_float(v[16 + 2 * i]),
+                                     skinny::siluOf(__uint_as_float(v[2 * i + 1])) * __uint_as_float(v[17 + 2 * i]));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = skinny::pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+            }
+#pragma unroll
+            for (int j = 0; j < kOutWords / 4; ++j) {
+              const uint32_t piece = uint32_t(c * (kOutWords / 4) + j);
+              tc::stShared16(buf + uint32_t(lane) * 64u + (piece ^ uint32_t(lane >> 1 & 3)) * 16u, o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            }
           }
           tc::fenceProxyAsyncShared();
           __syncwarp();
-          const int acc = w.col0 + (first + u) * 64;
+          const int acc = w.col0 + first * 64 + u * kChunks * 32;
           if (lane == 0) { tc::tmaStore2d(&maps.c, SWIGLU ? acc / 2 : acc, row0, buf); tc::bulkCommitGroup(); }
         }
       }
@@ -672,7 +672,7 @@ bool scaleMap(CUtensorMap* map, const void* ptr, int rows, int cols, int rowBloc
   return true;
 }
 // the output, in boxes of 32 rows x 64 bytes (32 columns)
-bool narrowOutputMap(CUtensorMap* map, void* ptr, uint64_t rows, uint64_t cols) {
+bool outputMap(CUtensorMap* map, void* ptr, uint64_t rows, uint64_t cols) {
   const TensorMapEncodeFn fn = tensorMapEncodeFn();
   if (reinterpret_cast<uintptr_t>(ptr) % 16 || cols * 2 % 16) { setError("TMA operands need 16-byte aligned base and row pitch"); return false; }
   const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols * 2};
@@ -772,8 +772,7 @@ int launchWide(const void* aData, const void* aScales, const void* wData, const 
   if (!makeTensorMap(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, aData, uint64_t(M), uint64_t(K) / 2, uint64_t(K) / 2, kBM) ||
       !makeTensorMap(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, wData, uint64_t(N), uint64_t(K) / 2, uint64_t(K) / 2, uint32_t(p.boxRows)) ||
       !scaleMap(&maps.sa, aScales, M, K, 1) || !scaleMap(&maps.sb, wScales, N, K, 2) ||
-      !(swiglu ? narrowOutputMap(&maps.c, C, uint64_t(M), uint64_t(outCols))
-               : makeTensorMap(&maps.c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, C, uint64_t(M), uint64_t(outCols) * 2, uint64_t(outCols) * 2, 32))) return 1;
+      !outputMap(&maps.c, C, uint64_t(M), uint64_t(outCols))) return 1;
   cfg.gridDim = dim3(unsigned(2 * std::min(pairs, p.items))); cfg.numAttrs = 2;
   return launched(cudaLaunchKernelEx(&cfg, kernel, maps, p)) ? 0 : 1;
 }

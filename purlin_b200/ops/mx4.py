@@ -105,16 +105,13 @@ def _check_dense(x: torch.Tensor):
         raise ValueError("operands must start on a 16-byte boundary")
 
 
-def _rows(x: torch.Tensor) -> int:
-    return x.numel() // x.shape[-1]
-
-
 def quantize_mx4(x: torch.Tensor) -> Mx4Tensor:
     """``x [..., cols]`` (bf16, fp16 or fp32, contiguous, cols a multiple of 32) as an ``Mx4Tensor`` of its rows. A block's power of two is that of its
     largest magnitude over 4, at least 2^-127; values are rounded to the nearest of the format, ties to the even code, and above 6 times the power
     to 6. A block that holds an infinity or a NaN stands for NaNs."""
     _check_dense(x)
-    rows, cols = _rows(x), x.shape[-1]
+    cols = x.shape[-1]
+    rows = x.numel() // cols
     q = Mx4Tensor._empty(rows, cols, x.device)
     if rows:
         lib = _lib()
@@ -130,31 +127,35 @@ def _product(a: Union[torch.Tensor, Mx4Tensor], w: Mx4Tensor, out: Optional[torc
     if not quantised:
         _check_dense(a)
     n, k = w.shape
-    if a.shape[-1] != k or a.device != w.device:
+    device = w.data.device
+    shape = a.shape
+    if shape[-1] != k or a.device != device:
         raise ValueError("a is [..., K] and w is [N, K], on one device")
     if n == 0 or n % (32 if epilogue == EPI_SWIGLU else 8):
         raise ValueError("the SwiGLU epilogue needs N to be a multiple of 32 (16 rows of gate and 16 of up in turn)" if epilogue == EPI_SWIGLU
                          else "N must be a multiple of 8")
-    rows, cols = (a.shape[0] if quantised else _rows(a)), n // 2 if epilogue == EPI_SWIGLU else n
-    shape = (*a.shape[:-1], cols)
+    rows = shape[0] if quantised else a.numel() // k
+    shape = (*shape[:-1], n // 2 if epilogue == EPI_SWIGLU else n)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=w.device)
+        out = a.new_empty(shape) if not quantised and a.dtype == torch.bfloat16 else torch.empty(shape, dtype=torch.bfloat16, device=device)
     elif out.dtype != torch.bfloat16:
         raise TypeError("out is a bf16 tensor")
-    elif tuple(out.shape) != shape or out.device != w.device or not out.is_contiguous() or out.data_ptr() % 16:
+    elif out.shape != shape or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"out is a contiguous tensor of {shape} on the operands' device")
     if rows == 0:
         return out
     lib = _lib()
-    with _on(w.device):
+    with _on(device):
         if quantised:
             rc = lib.purlin_mx4_gemm(a.data.data_ptr(), a.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k, epilogue,
                                      None, _stream(None))
         else:
-            work = torch.empty(rows * k // 2 + scale_bytes(rows, k), dtype=torch.uint8, device=w.device)
+            values = rows * k // 2                              # (a row is a multiple of 16 bytes)
+            work = w.data.new_empty(values + scale_bytes(rows, k))
             at = work.data_ptr()
-            rc = lib.purlin_mx4_linear(a.data_ptr(), TYPES[a.dtype], at, at + rows * k // 2, w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k,
+            rc = lib.purlin_mx4_linear(a.data_ptr(), TYPES[a.dtype], at, at + values, w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k,
                                        epilogue, None, _stream(None))
+    if rc:
         _native.check(lib, rc)
     return out
 
