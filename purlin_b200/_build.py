@@ -12,6 +12,7 @@ compiler or a network.
 Libraries:
   libpurlin_host.so   layout engine, tuning table, CPU interpreter (g++ only)
   libpurlin_cuda.so   contexts, collectives, fused kernels (nvcc, sm_100a) + the host half
+  _purlin_torch.so    operators on torch tensors (allocation, stream, autograd) around libpurlin_cuda.so
 """
 from __future__ import annotations
 
@@ -177,6 +178,32 @@ def build_fastcall(force: bool = False, verbose: bool = False) -> Path:
         flags, force, verbose)
 
 
+def torch_ops_name() -> str:
+    import sysconfig
+    return "_purlin_torch" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so")
+
+
+def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
+    """The extension that gives the operators their torch face (csrc/src/torch_ops.cpp), linked against the in-tree libpurlin_cuda.so and the
+    installed torch, whose version is part of the key."""
+    import sysconfig
+
+    import torch
+    build_cuda(force, verbose)
+    home = Path(torch.__file__).resolve().parent
+    src = CSRC / "src" / "torch_ops.cpp"
+    cuda_include = str(Path(_nvcc()).resolve().parent.parent / "include")
+    flags = ["-std=c++17", "-O2", "-fPIC", "-DTORCH_EXTENSION_NAME=_purlin_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-DPURLIN_TORCH_VERSION=\"{torch.__version__}\""]
+    inc = [f for d in (home / "include", home / "include/torch/csrc/api/include", cuda_include, sysconfig.get_paths()["include"], CSRC / "include") for f in ("-isystem", str(d))]
+    return _build_one(
+        torch_ops_name(), [src],
+        lambda s, o: ["g++", *flags, *inc, "-c", str(s), "-o", str(o)],
+        lambda objs, out: ["g++", "-shared", "-o", str(out), *map(str, objs), "-L", str(home / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+                           "-L", str(LIB_DIR), "-lpurlin_cuda", "-Xlinker", "-rpath", "-Xlinker", "$ORIGIN"],
+        flags, force, verbose)
+
+
 def build_cpp_tests(force: bool = False, verbose: bool = False, folder: str = "tests"):
     """The C++ test binaries (csrc/tests) or example programs (csrc/examples), linked against the in-tree libpurlin_cuda.so."""
     lib = build_cuda(force, verbose)
@@ -220,7 +247,7 @@ def build_examples(force: bool = False, verbose: bool = False):
 
 
 def build_all(force: bool = False, verbose: bool = False):
-    return (build_host(force, verbose), build_cuda(force, verbose), build_fastcall(force, verbose), *build_cpp_tests(force, verbose),
+    return (build_host(force, verbose), build_cuda(force, verbose), build_fastcall(force, verbose), build_torch_ops(force, verbose), *build_cpp_tests(force, verbose),
             *build_examples(force, verbose), *build_cpu_tests(force, verbose))
 
 

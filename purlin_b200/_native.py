@@ -171,6 +171,23 @@ def fast_call_fixed(lib):
     return _fastcall[1].call_fixed if _fastcall[0] is lib else lib.purlin_call_fixed
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The operators on torch tensors (csrc/src/torch_ops.cpp). Raises if the extension cannot be built or loaded."""
+    global _torch_ops
+    if _torch_ops is None:
+        import importlib.util
+        cuda()                                  # the extension is linked against this library
+        path = _resolve(_build.torch_ops_name(), _build.build_torch_ops)
+        spec = importlib.util.spec_from_file_location("_purlin_torch", str(path))
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        _torch_ops = mod
+    return _torch_ops
+
+
 def last_error(lib) -> str:
     return (lib.purlin_last_error() or b"").decode()
 

@@ -1,4 +1,4 @@
-"""4-bit microscaled tensors and products of them (csrc/src/mx4.cu).
+"""4-bit microscaled tensors and products of them (csrc/src/mx4.cu, csrc/src/torch_ops.cpp).
 
 32 neighbouring values of a row share a power of two (a byte, e8m0); each is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it, with a sign (e2m1): 4.25
 bits a value. ``quantize_mx4`` makes such a tensor, ``mx4_gemm`` and ``mx4_gemm_swiglu`` multiply activations with a weight that was quantised once;
@@ -6,36 +6,14 @@ both operands go to the block-scaled tensor cores as they are, sums are fp32. Fo
 """
 from __future__ import annotations
 
-import ctypes as C
-from contextlib import nullcontext
 from typing import Optional, Tuple, Union
 
 import torch
 
-from .. import _native, _stream
+from .. import _native
 
 EPI_STORE, EPI_SWIGLU = 0, 1
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_declared = False
-
-
-def _lib():
-    global _declared
-    lib = _native.cuda()
-    if not _declared:
-        vp, i = C.c_void_p, C.c_int
-        lib.purlin_mx4_scale_bytes.argtypes = [i, i]
-        lib.purlin_mx4_scale_bytes.restype = C.c_size_t
-        lib.purlin_mx4_quantize.argtypes = [vp, i, vp, vp, i, i, vp]
-        lib.purlin_mx4_dequantize.argtypes = [vp, vp, vp, i, i, i, vp]
-        lib.purlin_mx4_gemm.argtypes = [vp] * 5 + [i] * 4 + [vp, vp]
-        lib.purlin_mx4_linear.argtypes = [vp, i] + [vp] * 5 + [i] * 4 + [vp, vp]
-        _declared = True
-    return lib
-
-
-def _on(device: torch.device):
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def scale_bytes(rows: int, cols: int) -> int:
@@ -61,10 +39,9 @@ class Mx4Tensor:
         self.data, self.scales = data, scales
 
     @classmethod
-    def _empty(cls, rows: int, cols: int, device) -> "Mx4Tensor":
-        q = cls.__new__(cls)                 # (what it is made of needs no check)
-        q.data = torch.empty((rows, cols // 2), dtype=torch.uint8, device=device)
-        q.scales = torch.empty(scale_bytes(rows, cols), dtype=torch.uint8, device=device)
+    def _of(cls, data: torch.Tensor, scales: torch.Tensor) -> "Mx4Tensor":
+        q = cls.__new__(cls)                 # (what the quantisation made needs no check)
+        q.data, q.scales = data, scales
         return q
 
     @property
@@ -85,13 +62,7 @@ class Mx4Tensor:
         """The values that the tensor stands for, exact in ``dtype`` (bf16 or fp32)."""
         if dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("values come back in bf16 or fp32")
-        rows, cols = self.shape
-        out = torch.empty(rows, cols, dtype=dtype, device=self.device)
-        if rows:
-            lib = _lib()
-            with _on(self.device):
-                _native.check(lib, lib.purlin_mx4_dequantize(self.data.data_ptr(), self.scales.data_ptr(), out.data_ptr(), TYPES[dtype], rows, cols, _stream(None)))
-        return out
+        return _native.torch_ops().mx4_dequantize(self.data, self.scales, TYPES[dtype])
 
 
 def _check_dense(x: torch.Tensor):
@@ -111,13 +82,7 @@ def quantize_mx4(x: torch.Tensor) -> Mx4Tensor:
     to 6. A block that holds an infinity or a NaN stands for NaNs."""
     _check_dense(x)
     cols = x.shape[-1]
-    rows = x.numel() // cols
-    q = Mx4Tensor._empty(rows, cols, x.device)
-    if rows:
-        lib = _lib()
-        with _on(x.device):
-            _native.check(lib, lib.purlin_mx4_quantize(x.data_ptr(), TYPES[x.dtype], q.data.data_ptr(), q.scales.data_ptr(), rows, cols, _stream(None)))
-    return q
+    return Mx4Tensor._of(*_native.torch_ops().mx4_quantize(x, TYPES[x.dtype], x.numel() // cols, cols))
 
 
 def _product(a: Union[torch.Tensor, Mx4Tensor], w: Mx4Tensor, out: Optional[torch.Tensor], epilogue: int) -> torch.Tensor:
@@ -136,27 +101,15 @@ def _product(a: Union[torch.Tensor, Mx4Tensor], w: Mx4Tensor, out: Optional[torc
                          else "N must be a multiple of 8")
     rows = shape[0] if quantised else a.numel() // k
     shape = (*shape[:-1], n // 2 if epilogue == EPI_SWIGLU else n)
+    operand = (a.data, 0, a.scales) if quantised else (a, TYPES[a.dtype], None)
     if out is None:
-        out = a.new_empty(shape) if not quantised and a.dtype == torch.bfloat16 else torch.empty(shape, dtype=torch.bfloat16, device=device)
-    elif out.dtype != torch.bfloat16:
+        return _native.torch_ops().mx4_new_product(*operand, w.data, w.scales, shape, rows, epilogue)
+    if out.dtype != torch.bfloat16:
         raise TypeError("out is a bf16 tensor")
-    elif out.shape != shape or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
+    if out.shape != shape or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"out is a contiguous tensor of {shape} on the operands' device")
-    if rows == 0:
-        return out
-    lib = _lib()
-    with _on(device):
-        if quantised:
-            rc = lib.purlin_mx4_gemm(a.data.data_ptr(), a.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k, epilogue,
-                                     None, _stream(None))
-        else:
-            values = rows * k // 2                              # (a row is a multiple of 16 bytes)
-            work = w.data.new_empty(values + scale_bytes(rows, k))
-            at = work.data_ptr()
-            rc = lib.purlin_mx4_linear(a.data_ptr(), TYPES[a.dtype], at, at + values, w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k,
-                                       epilogue, None, _stream(None))
-    if rc:
-        _native.check(lib, rc)
+    if rows:
+        _native.torch_ops().mx4_product(*operand, w.data, w.scales, out, rows, epilogue)
     return out
 
 
