@@ -57,9 +57,10 @@ struct alignas(64) Group {
   int M, N, K, tilesM, tilesN;
   int aMn;                               // m is contiguous in A (k otherwise)
   int aBytes;                            // that one block of A brings into a stage: fewer than 128 rows of it where there are fewer
+  int split;                             // parts of k, a tile of work each; above 1 the sums go to `partial` and finishKernel adds them up
 };
-// Tiles [start, start + count) of a group (with `halves` their accumulators one by one, 2 * count of them) in turn over `pairs` CTA pairs (or CTAs)
-// from number `first` on, wrapping around.
+// Work [start, start + count) of a group (tiles, times the parts of k; with `halves` their accumulators one by one, 2 * count of them) in turn over
+// `pairs` CTA pairs (or CTAs) from number `first` on, wrapping around.
 struct Segment { int group, start, count, first, pairs, halves; };
 constexpr int kMaxGroups = 3, kMaxSegments = 3 * kMaxGroups;
 
@@ -71,6 +72,7 @@ struct alignas(64) Params {
   uint4* saved;                          // pre-activations: written by kGate (unless null), read by kGateGrad
   int savedCols;                         // its 32-column blocks per row block
   int activation;
+  float4* partial;                       // of the first group, where its k is split: [part][tile][accumulator, CTA, quarter][32 columns][8][32 lanes]
   uint32_t* status;
   uint64_t timeoutNs;
 };
@@ -169,7 +171,13 @@ PURLIN_D void tileCoord(const Group& g, int t, int& mIdx, int& nIdx) {
   nIdx = within / rows;
 }
 // first row of the pair's accumulators, first column, number of accumulators
-struct Item { int group, tile, row, col, count; };
+struct Item { int group, tile, part, row, col, count; };
+constexpr int kPartialBlock = 8 * 32;    // 32 rows x 32 columns of partial sums in 16-byte pieces: eight for every lane (a row), 512 bytes side by side
+struct KRange { int begin, end; };       // k-blocks of a part
+PURLIN_D KRange kRangeOf(const Group& g, int part) {
+  const int blocks = (g.K + kBK - 1) / kBK;
+  return KRange{int(int64_t(blocks) * part / g.split), int(int64_t(blocks) * (part + 1) / g.split)};
+}
 // The work of pair `idx` of `units`, in the order in which all warps walk it; body returns false to stop.
 template <int CTAS, int ACCS, typename F> PURLIN_D void forItems(const Params& p, int idx, int units, F&& body) {
   for (int s = 0; s < p.segments; ++s) {
@@ -183,6 +191,8 @@ template <int CTAS, int ACCS, typename F> PURLIN_D void forItems(const Params& p
       int mIdx, nIdx, first = 0;
       m.group = seg.group;
       m.tile = seg.start + (ACCS == 2 && seg.halves ? i >> 1 : i);
+      m.part = 0;
+      if (g.split > 1) { const int tiles = g.tilesM * g.tilesN; m.part = m.tile / tiles; m.tile -= m.part * tiles; }
       tileCoord(g, m.tile, mIdx, nIdx);
       m.count = 1;
       if constexpr (ACCS == 2) {
@@ -249,10 +259,11 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
     uint32_t st = 0, ph = 0;
     forItems<CTAS, ACCS>(p, pairIdx, numPairs, [&](const Item& m) {
       const Group& g = p.g[m.group];
-      const int aRow = m.row + int(ctaRank) * kBM, bRow = m.col + int(ctaRank) * bnLocal, kBlocks = (g.K + kBK - 1) / kBK;
+      const int aRow = m.row + int(ctaRank) * kBM, bRow = m.col + int(ctaRank) * bnLocal;
+      const KRange k = kRangeOf(g, m.part);
       const bool aMn = kAnyA && g.aMn;
       const uint32_t bytes = uint32_t(CTAS * (m.count * g.aBytes + bBytes));
-      for (int kb = 0; kb < kBlocks; ++kb) {
+      for (int kb = k.begin; kb < k.end; ++kb) {
         const bool ok = waitAll(emptyBar(st), ph ^ 1, abortWord, p.timeoutNs);
         if (!ok) { if (elected) skinny::recordTimeout(p.status, 1, m.tile, kb); return false; }
         if (elected) {
@@ -298,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
       uint32_t st = 0, ph = 0, accIt = 0, use0 = 0, use1 = 0;
       forItems<CTAS, ACCS>(p, pairIdx, numPairs, [&](const Item& m) {
         const Group& g = p.g[m.group];
-        const int kBlocks = (g.K + kBK - 1) / kBK;
+        const KRange range = kRangeOf(g, m.part);
         const int a0 = ACCS == 1 ? int(accIt & 1) : 0;
         const bool two = ACCS == 2 && m.count == 2;
         bool ok = waitAll(tmemEmptyBar(a0), ((a0 ? use1 : use0) & 1) ^ 1, abortWord, p.timeoutNs);
@@ -310,14 +321,14 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
           constexpr uint32_t kStepA = aMn ? kStepMn : kStepK;
           const uint32_t idesc = tc::instrDescBf16(uint32_t(p.bn), uint32_t(kBM * CTAS)) | (aMn ? tc::kInstrDescAMnMajor : 0u) | (B_MN ? tc::kInstrDescBMnMajor : 0u);
           const uint64_t descA0 = aMn ? tc::smemDescSw128MnMajor(base) : tc::smemDescSw128(base);
-          for (int kb = 0; kb < kBlocks; ++kb) {
+          for (int kb = range.begin; kb < range.end; ++kb) {
             ok = waitAll(fullBar(st), ph, abortWord, p.timeoutNs);
             if (!ok) { if (elected) skinny::recordTimeout(p.status, 3, m.tile, kb); return; }
             tc::fenceAfterThreadSync();
             const uint64_t off = uint64_t(st * stageStep), da = descA0 + off, db = descB0 + off;
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k) {
-              const uint32_t accumulate = uint32_t(kb != 0 || k != 0);
+              const uint32_t accumulate = uint32_t(kb != range.begin || k != 0);
               mma<CTAS>(elected, d0, da + kStepA * k, db + kStepB * k, idesc, accumulate);
               if constexpr (decltype(both)::value) mma<CTAS>(elected, d1, da + accStep + kStepA * k, db + kStepB * k, idesc, accumulate);
             }
@@ -378,7 +389,19 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
         __syncwarp();
         if (lane == 0) { tc::tmaStore2d(&g.c, col, row0, buf); tc::bulkCommitGroup(); }
       };
-      if constexpr (EPI == kGateGrad) {
+      if (EPI == kStore && g.split > 1) {
+        const size_t block = ((size_t(m.part) * size_t(g.tilesM * g.tilesN) + size_t(m.tile)) * (ACCS * CTAS) + size_t((m.row / (CTAS * kBM) % ACCS + (ACCS == 2 && m.count == 2 ? group : 0)) * CTAS + int(ctaRank))) * 4 + size_t(quarter);
+        float4* to = p.partial + block * size_t(p.bn / 32) * kPartialBlock + lane;
+#pragma unroll 1
+        for (int c = 0; c < nChunks; ++c) {
+          uint32_t r[32];
+          tc::tmemLoad32(taddr + uint32_t(c * 32), r);
+          tc::tmemLoadWaitFor(r);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            to[size_t(c) * kPartialBlock + i * 32] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+        }
+      } else if constexpr (EPI == kGateGrad) {
         // 32 columns of dh are 64 of dZ: [16 dG][16 dU][16 dG][16 dU], one staging tile
         const int blocks = min(p.bn, g.N - n0) / 16;                    // saved blocks of this tile (N is a multiple of 16)
 #pragma unroll 1
@@ -467,10 +490,52 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
   }
 }
 
+// The parts of a product whose k was split, added in ascending order of k: a warp per 32 rows x 32 columns, a row to a lane, as the epilogue
+// laid them down. (A second launch and not the last part's epilogue: one warp adding up sixteen parts takes far longer than all.)
+constexpr int kFinishThreads = 256;
+__global__ void __launch_bounds__(kFinishThreads) finishKernel(const float4* __restrict__ partial, __nv_bfloat16* __restrict__ out, int M, int N, int split, int tiles, int tilesM, int tilesN,
+                                                                int blocksM, int bn, int64_t warps) {
+  tc::gridDependencyWait();
+  tc::gridLaunchDependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t w = int64_t(blockIdx.x) * (kFinishThreads / 32) + (threadIdx.x >> 5);
+  if (w >= warps) return;
+  const int chunks = bn / 32, c = int(w % chunks);
+  const int64_t block = w / chunks;                            // tile, then accumulator, CTA and quarter: blocksM blocks of 32 rows
+  const int tile = int(block / blocksM), rowBlock = int(block % blocksM);
+  Group g;
+  g.tilesM = tilesM; g.tilesN = tilesN;
+  int mIdx, nIdx;
+  tileCoord(g, tile, mIdx, nIdx);
+  const int row = (mIdx * blocksM + rowBlock) * 32 + lane, col = nIdx * bn + c * 32;
+  if (row - lane >= M || col >= N) return;
+  const size_t stride = size_t(tiles) * size_t(blocksM) * size_t(chunks) * kPartialBlock;
+  const float4* from = partial + (size_t(block) * size_t(chunks) + size_t(c)) * kPartialBlock + lane;
+  float4 sum[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum[i] = __ldcs(from + i * 32);
+#pragma unroll 2
+  for (int s = 1; s < split; ++s) {
+    from += stride;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 v = __ldcs(from + i * 32);
+      sum[i].x += v.x; sum[i].y += v.y; sum[i].z += v.z; sum[i].w += v.w;
+    }
+  }
+  if (row >= M) return;
+  __nv_bfloat16* to = out + size_t(row) * size_t(N) + col;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)                                   // (N is a multiple of 8)
+    if (col + 8 * i < N)
+      *reinterpret_cast<uint4*>(to + 8 * i) = make_uint4(skinny::pack2(sum[2 * i].x, sum[2 * i].y), skinny::pack2(sum[2 * i].z, sum[2 * i].w),
+                                                         skinny::pack2(sum[2 * i + 1].x, sum[2 * i + 1].y), skinny::pack2(sum[2 * i + 1].z, sum[2 * i + 1].w));
+}
+
 // ------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------
-struct Shape { int ctas, accs, bn; };
+struct Shape { int ctas, accs, bn, split; };     // split: parts of the first product's k
 
 struct Device { int sms = 0, index = -1; };
 bool currentDevice(Device& d) {
@@ -498,35 +563,45 @@ double tileCycles(const Sizes& z, const Shape& s, int epi) {
   const double epilogue = s.bn * (s.accs == 2 ? 16.0 : 8.0) * (epi == kStore ? 1.0 : 2.0), main = kBlocks * std::max(mma, load);
   return s.accs == 2 ? main + 1500 + epilogue : std::max(main + 500, epilogue);
 }
-// The tile that is expected to take least.
-Shape chooseShape(const Sizes* z, int n, int sms, int epi) {
-  Shape best{2, 2, 256};
+size_t partialBytes(const Sizes& z, const Shape& s) { return s.split > 1 ? size_t(s.split) * size_t(tilesOf(z, s)) * size_t(kBM * s.ctas * s.accs) * size_t(s.bn) * 4 : 0; }
+constexpr int kMaxSplit = 16;
+constexpr size_t kMaxPartial = size_t(256) << 20;
+// The tile that is expected to take least, and the parts into which k of the first product is cut (where `mayCut`): its tiles may be few and long.
+// The gradient of x, [tokens, hidden], sums over twice the intermediate size: 2595 x 424 with k = 46560 has 12 tiles (all three gradients, us, whole /
+// cut: 2595, 424, 23280 375 / 281; 16, 8192, 28672 530 / 511; 100, 1024, 2048 22.0 / 16.9).
+Shape chooseShape(const Sizes* z, int n, int sms, int epi, bool mayCut) {
+  Shape best{2, 2, 256, 1};
   double least = 1e30;
   auto consider = [&](Shape s) {
     const int units = sms / s.ctas;
-    double cycles = 0, longest = 0;
-    if (n == 1) {
-      const int64_t tiles = tilesOf(z[0], s), rest = tiles % units;
-      double waves = double((tiles + units - 1) / units);
-      if (s.accs == 2 && tiles > units && rest > 0 && 2 * rest <= units) waves -= 0.5;
-      cycles = waves * tileCycles(z[0], s, epi);
-    } else {
-      double last = 0;
-      for (int i = 0; i < n; ++i) {
-        last = tileCycles(z[i], s, epi);
-        longest = std::max(longest, last);
-        cycles += double(tilesOf(z[i], s)) * last / units;
+    for (s.split = 1; s.split <= (mayCut ? kMaxSplit : 1); s.split *= 2) {
+      const Sizes first{z[0].M, z[0].N, (z[0].K + s.split - 1) / s.split};
+      if (s.split > 1 && (first.K < 4 * kBK || partialBytes(z[0], s) > kMaxPartial)) break;
+      double cycles = 0, longest = 0;
+      if (n == 1) {
+        const int64_t tiles = tilesOf(z[0], s) * s.split, rest = tiles % units;
+        double waves = double((tiles + units - 1) / units);
+        if (s.accs == 2 && tiles > units && rest > 0 && 2 * rest <= units) waves -= 0.5;
+        cycles = waves * tileCycles(first, s, epi);
+      } else {
+        double last = 0;
+        for (int i = 0; i < n; ++i) {
+          last = tileCycles(i ? z[i] : first, s, epi);
+          longest = std::max(longest, last);
+          cycles += double(tilesOf(z[i], s)) * (i ? 1 : s.split) * last / units;
+        }
+        cycles = std::max(cycles + 0.5 * last, longest);
       }
-      cycles = std::max(cycles + 0.5 * last, longest);
+      if (s.accs == 1) cycles += 1500 + s.bn * 8.0;
+      if (s.split > 1) cycles += 6000 + double(partialBytes(z[0], s)) / 1500;     // a launch, and the parts written and read at about 3000 bytes a cycle
+      if (cycles < least) { least = cycles; best = s; }
     }
-    if (s.accs == 1) cycles += 1500 + s.bn * 8.0;
-    if (cycles < least) { least = cycles; best = s; }
   };
-  consider({2, 2, 256});
-  consider({2, 2, 128});
-  consider({1, 1, 256});
-  consider({1, 1, 128});
-  if (epi != kGate) consider({1, 1, 64});     // (64 columns of Z are 32 of h: half a staging tile)
+  consider({2, 2, 256, 1});
+  consider({2, 2, 128, 1});
+  consider({1, 1, 256, 1});
+  consider({1, 1, 128, 1});
+  if (epi != kGate) consider({1, 1, 64, 1});     // (64 columns of Z are 32 of h: half a staging tile)
   return best;
 }
 
@@ -535,7 +610,7 @@ Shape chooseShape(const Sizes* z, int n, int sms, int epi) {
 void shareOut(Params& p, int groups, const Shape& s, int units, int epi) {
   int order[kMaxGroups] = {0, 1, 2};
   double cost[kMaxGroups] = {};
-  for (int i = 0; i < groups; ++i) cost[i] = tileCycles(Sizes{p.g[i].M, p.g[i].N, p.g[i].K}, s, epi);
+  for (int i = 0; i < groups; ++i) cost[i] = tileCycles(Sizes{p.g[i].M, p.g[i].N, (p.g[i].K + p.g[i].split - 1) / p.g[i].split}, s, epi);
   std::sort(order, order + groups, [&](int a, int b) { return cost[a] > cost[b]; });
   int lateFirst = 0, late = 0;                // pairs [lateFirst, lateFirst + late), wrapping around, end `ahead` cycles after the others
   double ahead = 0;
@@ -544,7 +619,7 @@ void shareOut(Params& p, int groups, const Shape& s, int units, int epi) {
   };
   p.segments = 0;
   for (int i = 0; i < groups; ++i) {
-    const int group = order[i], tiles = p.g[group].tilesM * p.g[group].tilesN;
+    const int group = order[i], tiles = p.g[group].tilesM * p.g[group].tilesN * p.g[group].split;
     int done = 0;
     if (late > 0) {
       const int each = int(ahead / cost[group] + 0.5);
@@ -595,8 +670,8 @@ int launchAs(Params& p, int groups, const Shape& s, const Device& dev, cudaStrea
     const Sizes z{p.g[i].M, p.g[i].N, p.g[i].K};
     const int tileRows = kBM * CTAS * ACCS;
     p.g[i].tilesM = (z.M + tileRows - 1) / tileRows; p.g[i].tilesN = (z.N + s.bn - 1) / s.bn;
-    if (tilesOf(z, s) > INT32_MAX / 4) { setError("feed-forward: the product is too large"); return 1; }
-    tiles += tilesOf(z, s);
+    if (tilesOf(z, s) * p.g[i].split > INT32_MAX / 4) { setError("feed-forward: the product is too large"); return 1; }
+    tiles += tilesOf(z, s) * p.g[i].split;
   }
   units = int(std::min<int64_t>(units, tiles));
   shareOut(p, groups, s, units, EPI);
@@ -614,16 +689,21 @@ int launchAs(Params& p, int groups, const Shape& s, const Device& dev, cudaStrea
 
 // C[M, N] (or the gated forms) = sum over k of A(m, k) B(n, k). A is [M, K] row-major, or [K, M] with aMn; B is [N, K], or [K, N] with B_MN.
 struct Product { const void *A, *B; void* C; int M, N, K; bool aMn; };
+Shape shapeOf(const Product* products, int n, const Device& dev, int epi, bool mayCut) {
+  Sizes z[kMaxGroups] = {};
+  for (int i = 0; i < n; ++i) z[i] = Sizes{products[i].M, products[i].N, products[i].K};
+  return chooseShape(z, n, dev.sms, epi, mayCut);
+}
+// `partial`: room for the parts of the first product's k, or null where it is not to be cut
 template <bool B_MN, int EPI>
-int run(const Product* products, int n, void* saved, int activation, uint32_t* status, cudaStream_t stream) {
+int run(const Product* products, int n, void* saved, void* partial, int activation, uint32_t* status, cudaStream_t stream) {
   Device dev;
   if (!currentDevice(dev)) return 1;
   Params p{};
-  Sizes z[kMaxGroups] = {};
-  for (int i = 0; i < n; ++i) z[i] = Sizes{products[i].M, products[i].N, products[i].K};
-  const Shape s = chooseShape(z, n, dev.sms, EPI);
+  const Shape s = shapeOf(products, n, dev, EPI, partial != nullptr);
   p.bn = s.bn;
-  p.saved = static_cast<uint4*>(saved); p.savedCols = EPI == kGate ? z[0].N / 32 : z[0].N / 16;
+  p.partial = static_cast<float4*>(partial);
+  p.saved = static_cast<uint4*>(saved); p.savedCols = EPI == kGate ? products[0].N / 32 : products[0].N / 16;
   p.activation = activation; p.status = status; p.timeoutNs = 2ull * 1000 * 1000 * 1000;
   auto bf16Map = [](CUtensorMap& m, const void* ptr, int rows, int cols, int boxRows) {
     return makeTensorMap(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ptr, uint64_t(rows), uint64_t(cols) * 2, uint64_t(cols) * 2, uint32_t(boxRows));
@@ -631,7 +711,7 @@ int run(const Product* products, int n, void* saved, int activation, uint32_t* s
   for (int i = 0; i < n; ++i) {
     const Product& q = products[i];
     Group& g = p.g[i];
-    g.M = q.M; g.N = q.N; g.K = q.K; g.aMn = q.aMn;
+    g.M = q.M; g.N = q.N; g.K = q.K; g.aMn = q.aMn; g.split = i ? 1 : s.split;
     // Few rows of A take only their own room in a stage: the MMA's other rows read what lies behind, and rows of the accumulator that are no
     // rows of the result are never stored.
     const int boxRows = q.aMn || s.ctas == 2 ? kBM : std::min(kBM, (q.M + 7) / 8 * 8);
@@ -643,7 +723,29 @@ int run(const Product* products, int n, void* saved, int activation, uint32_t* s
   }
   const int stageBytes = s.accs * p.aBytes + s.bn / s.ctas * kBK * 2;
   p.stages = std::min((kSmemLimit - kBarrierBytes - 1024 - kStagingBytes) / stageBytes, kMaxStages);
-  return s.ctas == 2 ? launchAs<B_MN, EPI, 2, 2>(p, n, s, dev, stream) : launchAs<B_MN, EPI, 1, 1>(p, n, s, dev, stream);
+  const int rc = s.ctas == 2 ? launchAs<B_MN, EPI, 2, 2>(p, n, s, dev, stream) : launchAs<B_MN, EPI, 1, 1>(p, n, s, dev, stream);
+  if (rc || s.split == 1) return rc;
+  const Group& g = p.g[0];
+  const int blocksM = s.ctas * s.accs * 4, tiles = g.tilesM * g.tilesN;
+  const int64_t warps = int64_t(tiles) * blocksM * (s.bn / 32);
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(unsigned((warps + kFinishThreads / 32 - 1) / (kFinishThreads / 32))); cfg.blockDim = dim3(kFinishThreads); cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, finishKernel, static_cast<const float4*>(p.partial), static_cast<__nv_bfloat16*>(products[0].C), g.M, g.N, g.split, tiles, g.tilesM, g.tilesN,
+                                           blocksM, s.bn, warps);
+  if (e != cudaSuccess) { setError(std::string("feed-forward launch: ") + cudaGetErrorString(e)); return 1; }
+  return 0;
+}
+
+// the gradients that are wanted, dx first
+int gradients(Product (&g)[kMaxGroups], const void* x, const void* wGateUp, const void* h, const void* dy, const void* dz, void* dx, void* dGateUp, void* dDown, int tokens, int hidden,
+              int intermediate) {
+  int n = 0;
+  if (dx) g[n++] = Product{dz, wGateUp, dx, tokens, hidden, 2 * intermediate, false};
+  if (dGateUp) g[n++] = Product{dz, x, dGateUp, 2 * intermediate, hidden, tokens, true};
+  if (dDown) g[n++] = Product{dy, h, dDown, hidden, intermediate, tokens, true};
+  return n;
 }
 
 bool sizesFit(int tokens, int hidden, int intermediate, int activation) {
@@ -671,27 +773,33 @@ int purlin_ffn_forward(const void* x, const void* wGateUp, const void* wDown, vo
   const Product up{x, wGateUp, hOut, tokens, 2 * intermediate, hidden, false};
   const int rc = !saved && activation == PURLIN_ACT_SILU
       ? purlin_gemm_bf16(x, wGateUp, hOut, tokens, 2 * intermediate, hidden, PURLIN_EPI_SWIGLU, 0, status, stream)
-      : run<false, kGate>(&up, 1, saved, activation, status, static_cast<cudaStream_t>(stream));
+      : run<false, kGate>(&up, 1, saved, nullptr, activation, status, static_cast<cudaStream_t>(stream));
   if (rc || !y) return rc;
   return purlin_gemm_bf16(hOut, wDown, y, tokens, hidden, intermediate, PURLIN_EPI_STORE, 0, status, stream);
 }
 
 int purlin_ffn_backward(const void* x, const void* wGateUp, const void* wDown, const void* h, const void* saved, const void* dy, void* dz,
-                        void* dx, void* dGateUp, void* dDown, int tokens, int hidden, int intermediate, int activation, uint32_t* status, void* stream) {
+                        void* dx, void* dGateUp, void* dDown, void* workspace, int tokens, int hidden, int intermediate, int activation, uint32_t* status, void* stream) {
   NvtxRange range("ffnBackward", size_t(tokens) * size_t(hidden) * 2);
   if (!sizesFit(tokens, hidden, intermediate, activation)) return 1;
-  if (reinterpret_cast<uintptr_t>(saved) % 16) { setError("feed-forward: the saved pre-activations need 16-byte alignment"); return 1; }
+  if ((reinterpret_cast<uintptr_t>(saved) | reinterpret_cast<uintptr_t>(workspace)) % 16) { setError("feed-forward: the saved pre-activations and the workspace need 16-byte alignment"); return 1; }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dx || dGateUp) {
     const Product gradZ{dy, wDown, dz, tokens, intermediate, hidden, false};
-    if (run<true, kGateGrad>(&gradZ, 1, const_cast<void*>(saved), activation, status, s)) return 1;
+    if (run<true, kGateGrad>(&gradZ, 1, const_cast<void*>(saved), nullptr, activation, status, s)) return 1;
   }
   Product grads[kMaxGroups];
-  int n = 0;
-  if (dx) grads[n++] = Product{dz, wGateUp, dx, tokens, hidden, 2 * intermediate, false};
-  if (dGateUp) grads[n++] = Product{dz, x, dGateUp, 2 * intermediate, hidden, tokens, true};
-  if (dDown) grads[n++] = Product{dy, h, dDown, hidden, intermediate, tokens, true};
-  return n ? run<true, kStore>(grads, n, nullptr, activation, status, s) : 0;
+  const int n = gradients(grads, x, wGateUp, h, dy, dz, dx, dGateUp, dDown, tokens, hidden, intermediate);
+  return n ? run<true, kStore>(grads, n, nullptr, dx ? workspace : nullptr, activation, status, s) : 0;
+}
+
+size_t purlin_ffn_workspace_bytes(int tokens, int hidden, int intermediate, int wantDx, int wantGateUp, int wantDown) {
+  Device dev;
+  if (!wantDx || tokens <= 0 || hidden <= 0 || intermediate <= 0 || !currentDevice(dev)) return 0;
+  Product grads[kMaxGroups];
+  void* some = grads;                   // (sizes only)
+  const int n = gradients(grads, some, some, some, some, some, some, wantGateUp ? some : nullptr, wantDown ? some : nullptr, tokens, hidden, intermediate);
+  return partialBytes(Sizes{grads[0].M, grads[0].N, grads[0].K}, shapeOf(grads, n, dev, kStore, true));
 }
 
 }  // extern "C"

@@ -70,7 +70,9 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
         Tensor dy = grads[0].contiguous();
         if (reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16) dy = dy.clone();
         if (needs & 3) dz = at::empty({tokens, 2 * intermediate}, x.options());
-        check(purlin_ffn_backward(x.data_ptr(), wGateUp.data_ptr(), wDown.data_ptr(), ptr(h), ptr(saved), dy.data_ptr(), ptr(dz), ptr(dx), ptr(dGateUp), ptr(dDown), int(tokens),
+        Tensor work;
+        if (const size_t n = purlin_ffn_workspace_bytes(int(tokens), int(hidden), int(intermediate), int(needs & 1), int(needs & 2), int(needs & 4))) work = bytes(int64_t(n), x);
+        check(purlin_ffn_backward(x.data_ptr(), wGateUp.data_ptr(), wDown.data_ptr(), ptr(h), ptr(saved), dy.data_ptr(), ptr(dz), ptr(dx), ptr(dGateUp), ptr(dDown), ptr(work), int(tokens),
                                   int(hidden), int(intermediate), int(ctx->saved_data["activation"].toInt()), nullptr, stream()));
       }
     }

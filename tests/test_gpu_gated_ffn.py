@@ -67,7 +67,8 @@ NAMES = ("y", "dx", "dw_gu", "dw_down")
 
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
 @pytest.mark.parametrize("t,h,i", [(1, 8, 16), (1, 264, 176), (7, 72, 48), (40, 264, 176), (64, 1024, 512), (127, 200, 144), (128, 136, 272), (129, 520, 1040),
-                                   (333, 776, 336), (513, 1000, 528), (1100, 2048, 784), (2051, 264, 1296)])
+                                   (333, 776, 336), (513, 1000, 528), (1100, 2048, 784), (2051, 264, 1296),
+                                   (1, 1024, 4096), (100, 1024, 2048), (300, 424, 8192), (700, 136, 10000), (1500, 264, 4096)])   # few tiles, long sums: dx in parts
 def test_outputs_and_gradients_against_64_bits(t, h, i, activation):
     args = _inputs(t, h, i, seed=t + h + i)
     want, off = _oracle(*args, activation)
