@@ -81,9 +81,9 @@ PURLIN_D float sigmoidOf(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 // act(g) = g sigmoid(s(g)): s = g (silu), s = 2 sqrt(2 / pi) (g + 0.044715 g^3) (gelu with the tanh). Past |g| = 16 the sigmoid is 0 or 1
 // in fp32, so the cube is taken of the clamped value and cannot overflow.
 constexpr float kGeluScale = 1.5957691216057308f, kGeluCube = 0.044715f;
-PURLIN_D void activate(int activation, float g, float& act, float& grad) {
+template <int ACT> PURLIN_D void activate(float g, float& act, float& grad) {
   float s = g, ds = 1.f;
-  if (activation == PURLIN_ACT_GELU) {
+  if constexpr (ACT == PURLIN_ACT_GELU) {
     const float c = fminf(fmaxf(g, -16.f), 16.f), c2 = c * c;
     s = kGeluScale * c * fmaf(kGeluCube, c2, 1.f);
     ds = kGeluScale * fmaf(3.f * kGeluCube, c2, 1.f);
@@ -122,17 +122,26 @@ PURLIN_D void loadSaved(const uint4* block, int lane, uint32_t (&w)[24]) {
   }
 }
 
+template <int ACT> PURLIN_D void gate(const uint32_t (&r)[32], uint32_t (&o)[8]) {      // act(gate) * up of 32 columns (16 of each), packed to bf16
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float a0, a1, unused;
+    activate<ACT>(__uint_as_float(r[2 * i]), a0, unused);
+    activate<ACT>(__uint_as_float(r[2 * i + 1]), a1, unused);
+    o[i] = skinny::pack2(a0 * __uint_as_float(r[16 + 2 * i]), a1 * __uint_as_float(r[17 + 2 * i]));
+  }
+}
 // dG (o[0..7]) and dU (o[8..15]) of 16 columns, packed to bf16, from dh (columns C0 ... of the 32 in r) and the saved block
-template <int C0, int J = 0>
-PURLIN_D void gateGrad(int activation, const uint32_t (&r)[32], const uint32_t (&w)[24], uint32_t (&o)[16]) {
+template <int ACT, int C0, int J = 0>
+PURLIN_D void gateGrad(const uint32_t (&r)[32], const uint32_t (&w)[24], uint32_t (&o)[16]) {
   if constexpr (J < 16) {
     float a0, d0, a1, d1;
-    activate(activation, unpack24<J>(w), a0, d0);
-    activate(activation, unpack24<J + 1>(w), a1, d1);
+    activate<ACT>(unpack24<J>(w), a0, d0);
+    activate<ACT>(unpack24<J + 1>(w), a1, d1);
     const float h0 = __uint_as_float(r[C0 + J]), h1 = __uint_as_float(r[C0 + J + 1]);
     o[J / 2] = skinny::pack2(h0 * unpack24<16 + J>(w) * d0, h1 * unpack24<17 + J>(w) * d1);
     o[8 + J / 2] = skinny::pack2(h0 * a0, h1 * a1);
-    gateGrad<C0, J + 2>(activation, r, w, o);
+    gateGrad<ACT, C0, J + 2>(r, w, o);
   }
 }
 
@@ -365,11 +374,15 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
       // chunks of 32 accumulator columns that hold output
       const int nChunks = rowsValid <= 0 ? 0 : (min(p.bn, g.N - n0) + 31) / 32;
       uint4* saved = nullptr;                                           // of this warp's rows and the tile's first columns
-      uint32_t z[24];
+      uint32_t z[24], z1[24] = {};
+      const int blocks = min(p.bn, g.N - n0) / 16;                      // kGateGrad: saved blocks of this tile (N is a multiple of 16)
       if constexpr (EPI == kGate) { if (p.saved) saved = p.saved + (size_t(row0 / 32) * size_t(p.savedCols) + size_t(n0 / 32)) * (kSavedBlock / 16); }
       if constexpr (EPI == kGateGrad) {
         saved = p.saved + (size_t(row0 / 32) * size_t(p.savedCols) + size_t(n0 / 16)) * (kSavedBlock / 16);
-        if (nChunks > 0) loadSaved(saved, lane, z);                     // on the way while the tile's last MMAs run
+        if (nChunks > 0) {                                              // (a warp without rows has no saved blocks)
+          loadSaved(saved, lane, z);                                    // on the way while the tile's last MMAs run
+          if (blocks > 1) loadSaved(saved + kSavedBlock / 16, lane, z1);
+        }
       }
       if (!waitAll(tmemFullBar(group), uses & 1, abortWord, p.timeoutNs)) { if (lane == 0) skinny::recordTimeout(p.status, 5, m.tile, group); return false; }
       ++uses;
@@ -402,22 +415,24 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
             to[size_t(c) * kPartialBlock + i * 32] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
         }
       } else if constexpr (EPI == kGateGrad) {
-        // 32 columns of dh are 64 of dZ: [16 dG][16 dU][16 dG][16 dU], one staging tile
-        const int blocks = min(p.bn, g.N - n0) / 16;                    // saved blocks of this tile (N is a multiple of 16)
+        // 32 columns of dh are 64 of dZ: [16 dG][16 dU][16 dG][16 dU], one staging tile. The saved blocks of the next 32 are on the way meanwhile.
+        uint32_t r[32];
+        if (nChunks > 0) tc::tmemLoad32(taddr, r);
 #pragma unroll 1
         for (int c = 0; c < nChunks; ++c) {
-          uint32_t r[32], o[16];
-          tc::tmemLoad32(taddr + uint32_t(c * 32), r);
+          uint32_t o[32];
           const uint32_t buf = stagingTile();
           tc::tmemLoadWaitFor(r);
-          gateGrad<0>(p.activation, r, z, o);
-          if (2 * c + 1 < blocks) loadSaved(saved + size_t(2 * c + 1) * (kSavedBlock / 16), lane, z);
+          uint32_t (&o0)[16] = *reinterpret_cast<uint32_t (*)[16]>(o), (&o1)[16] = *reinterpret_cast<uint32_t (*)[16]>(o + 16);
+          if (p.activation == PURLIN_ACT_GELU) { gateGrad<PURLIN_ACT_GELU, 0>(r, z, o0); gateGrad<PURLIN_ACT_GELU, 16>(r, z1, o1); }
+          else { gateGrad<PURLIN_ACT_SILU, 0>(r, z, o0); gateGrad<PURLIN_ACT_SILU, 16>(r, z1, o1); }
+          if (c + 1 < nChunks) {
+            tc::tmemLoad32(taddr + uint32_t((c + 1) * 32), r);
+            loadSaved(saved + size_t(2 * c + 2) * (kSavedBlock / 16), lane, z);
+            if (2 * c + 3 < blocks) loadSaved(saved + size_t(2 * c + 3) * (kSavedBlock / 16), lane, z1);
+          }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) put(buf, j, o + 4 * j);
-          if (2 * c + 1 < blocks) gateGrad<16>(p.activation, r, z, o);  // (else these columns are past the output)
-          if (2 * c + 2 < blocks) loadSaved(saved + size_t(2 * c + 2) * (kSavedBlock / 16), lane, z);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) put(buf, 4 + j, o + 4 * j);
+          for (int j = 0; j < 8; ++j) put(buf, j, o + 4 * j);
           drain(buf, 2 * n0 + c * 64);
         }
       } else {
@@ -437,13 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
 #pragma unroll
                 for (int i = 0; i < kSavedVectors; ++i) __stcs(to + i * 32, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
               }
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                float a0, a1, unused;
-                activate(p.activation, __uint_as_float(r[2 * i]), a0, unused);
-                activate(p.activation, __uint_as_float(r[2 * i + 1]), a1, unused);
-                o[i] = skinny::pack2(a0 * __uint_as_float(r[16 + 2 * i]), a1 * __uint_as_float(r[17 + 2 * i]));
-              }
+              if (p.activation == PURLIN_ACT_GELU) gate<PURLIN_ACT_GELU>(r, o); else gate<PURLIN_ACT_SILU>(r, o);
             } else {
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = skinny::pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
@@ -553,15 +562,17 @@ int64_t tilesOf(const Sizes& z, const Shape& s) {
   const int tileRows = kBM * s.ctas * s.accs;
   return int64_t((z.M + tileRows - 1) / tileRows) * ((z.N + s.bn - 1) / s.bn);
 }
-// Expected cycles of a tile. A k-block (64 of k) takes the longest of its MMAs (bn / 2 cycles per 16 of k and accumulator, more where they
-// all go into one accumulator) and its loads from L2 (about 56 bytes a cycle and SM); a tile adds its epilogue, which with one
-// accumulator per tile hides under the next one's main loop.
+// Expected cycles of a tile. A k-block (64 of k) takes the longer of its MMAs (bn / 2 cycles per 16 of k and accumulator, a little more where they
+// all go into one) and its loads from L2 (about 56 bytes a cycle and SM). The epilogue follows the main loop of a tile of two accumulators and
+// hides under the next one's with one. us under the power cap, 512 x 256 / 256 x 256 per pair / 128 x 256 per CTA: gradient of the gate 1000 x 3584,
+// k 8192 99 / 66 / 79; 8192 x 4096, k 1024 124 / 113 / 110; gate and up 4099 x 4096, k 7168 201 / 216 / 262; 2595 x 46560, k 424 196 / 183 / 219.
 double tileCycles(const Sizes& z, const Shape& s, int epi) {
   const double kBlocks = (z.K + kBK - 1) / kBK;
-  const double mma = 4.0 * s.accs * s.bn / 2 * (s.accs == 2 ? 1.0 : 1.36);
+  const double mma = 4.0 * s.accs * s.bn / 2 * (s.accs == 2 ? 1.0 : 1.08);
   const double load = (s.accs * std::min(z.M, kBM) + s.bn / s.ctas) * 128.0 / 56;
-  const double epilogue = s.bn * (s.accs == 2 ? 16.0 : 8.0) * (epi == kStore ? 1.0 : 2.0), main = kBlocks * std::max(mma, load);
-  return s.accs == 2 ? main + 1500 + epilogue : std::max(main + 500, epilogue);
+  const double column = epi == kStore ? (s.accs == 2 ? 16 : 10) : epi == kGate ? (s.accs == 2 ? 46 : s.ctas == 2 ? 40 : 50) : s.accs == 2 ? 140 : s.ctas == 2 ? 75 : 80;
+  const double epilogue = s.bn * column, main = kBlocks * std::max(mma, load);
+  return s.accs == 2 ? main + 1500 + epilogue : std::max(main + 500, epilogue + 1200);
 }
 size_t partialBytes(const Sizes& z, const Shape& s) { return s.split > 1 ? size_t(s.split) * size_t(tilesOf(z, s)) * size_t(kBM * s.ctas * s.accs) * size_t(s.bn) * 4 : 0; }
 constexpr int kMaxSplit = 16;
@@ -593,12 +604,13 @@ Shape chooseShape(const Sizes* z, int n, int sms, int epi, bool mayCut) {
         cycles = std::max(cycles + 0.5 * last, longest);
       }
       if (s.accs == 1) cycles += 1500 + s.bn * 8.0;
-      if (s.split > 1) cycles += 6000 + double(partialBytes(z[0], s)) / 1500;     // a launch, and the parts written and read at about 3000 bytes a cycle
+      if (s.split > 1) cycles += 4000 + double(partialBytes(z[0], s)) / 3000;     // a launch, and the parts written and read
       if (cycles < least) { least = cycles; best = s; }
     }
   };
   consider({2, 2, 256, 1});
   consider({2, 2, 128, 1});
+  consider({2, 1, 256, 1});
   consider({1, 1, 256, 1});
   consider({1, 1, 128, 1});
   if (epi != kGate) consider({1, 1, 64, 1});     // (64 columns of Z are 32 of h: half a staging tile)
@@ -723,7 +735,8 @@ int run(const Product* products, int n, void* saved, void* partial, int activati
   }
   const int stageBytes = s.accs * p.aBytes + s.bn / s.ctas * kBK * 2;
   p.stages = std::min((kSmemLimit - kBarrierBytes - 1024 - kStagingBytes) / stageBytes, kMaxStages);
-  const int rc = s.ctas == 2 ? launchAs<B_MN, EPI, 2, 2>(p, n, s, dev, stream) : launchAs<B_MN, EPI, 1, 1>(p, n, s, dev, stream);
+  const int rc = s.accs == 2 ? launchAs<B_MN, EPI, 2, 2>(p, n, s, dev, stream)
+               : s.ctas == 2 ? launchAs<B_MN, EPI, 2, 1>(p, n, s, dev, stream) : launchAs<B_MN, EPI, 1, 1>(p, n, s, dev, stream);
   if (rc || s.split == 1) return rc;
   const Group& g = p.g[0];
   const int blocksM = s.ctas * s.accs * 4, tiles = g.tilesM * g.tilesN;
