@@ -21,11 +21,12 @@ int purlin_ffn_forward(const void* x, const void* wGateUp, const void* wDown, vo
 
 /* Gradients for dy [tokens, hidden]; h and saved from the forward. dz [tokens, 2 I]: workspace that holds the gradient of the
  * pre-activations (interleaved like wGateUp's rows). dx, dGateUp, dDown: any of them may be NULL and is then not computed; where neither dx nor
- * dGateUp is wanted, wDown, saved and dz are not touched. workspace: purlin_ffn_workspace_bytes() for the same gradients on the current device, or NULL
- * (dx may then take longer). */
+ * dGateUp is wanted, wDown, saved and dz are not touched. workspace: as many bytes as purlin_ffn_workspace_bytes() says for the same gradients
+ * on the current device; with fewer, or NULL, dx may take longer. */
 size_t purlin_ffn_workspace_bytes(int tokens, int hidden, int intermediate, int wantDx, int wantGateUp, int wantDown);
 int purlin_ffn_backward(const void* x, const void* wGateUp, const void* wDown, const void* h, const void* saved, const void* dy, void* dz,
-                        void* dx, void* dGateUp, void* dDown, void* workspace, int tokens, int hidden, int intermediate, int activation, uint32_t* status, void* stream);
+                        void* dx, void* dGateUp, void* dDown, void* workspace, size_t workspaceBytes, int tokens, int hidden, int intermediate,
+                        int activation, uint32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -783,6 +783,7 @@ int purlin_ffn_forward(const void* x, const void* wGateUp, const void* wDown, vo
   NvtxRange range("ffnForward", size_t(tokens) * size_t(hidden) * 2);
   if (!sizesFit(tokens, hidden, intermediate, activation)) return 1;
   if (reinterpret_cast<uintptr_t>(saved) % 16) { setError("feed-forward: the saved pre-activations need 16-byte alignment"); return 1; }
+  if (!x || !wGateUp || !hOut || (y && !wDown)) { setError("feed-forward: an operand is missing"); return 1; }
   const Product up{x, wGateUp, hOut, tokens, 2 * intermediate, hidden, false};
   const int rc = !saved && activation == PURLIN_ACT_SILU
       ? purlin_gemm_bf16(x, wGateUp, hOut, tokens, 2 * intermediate, hidden, PURLIN_EPI_SWIGLU, 0, status, stream)
@@ -792,10 +793,12 @@ int purlin_ffn_forward(const void* x, const void* wGateUp, const void* wDown, vo
 }
 
 int purlin_ffn_backward(const void* x, const void* wGateUp, const void* wDown, const void* h, const void* saved, const void* dy, void* dz,
-                        void* dx, void* dGateUp, void* dDown, void* workspace, int tokens, int hidden, int intermediate, int activation, uint32_t* status, void* stream) {
+                        void* dx, void* dGateUp, void* dDown, void* workspace, size_t workspaceBytes, int tokens, int hidden, int intermediate, int activation, uint32_t* status,
+                        void* stream) {
   NvtxRange range("ffnBackward", size_t(tokens) * size_t(hidden) * 2);
   if (!sizesFit(tokens, hidden, intermediate, activation)) return 1;
   if ((reinterpret_cast<uintptr_t>(saved) | reinterpret_cast<uintptr_t>(workspace)) % 16) { setError("feed-forward: the saved pre-activations and the workspace need 16-byte alignment"); return 1; }
+  if (!dy || ((dx || dGateUp) && (!wDown || !saved || !dz)) || (dx && !wGateUp) || (dGateUp && !x) || (dDown && !h)) { setError("feed-forward: an operand of a gradient is missing"); return 1; }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dx || dGateUp) {
     const Product gradZ{dy, wDown, dz, tokens, intermediate, hidden, false};
@@ -803,7 +806,9 @@ int purlin_ffn_backward(const void* x, const void* wGateUp, const void* wDown, c
   }
   Product grads[kMaxGroups];
   const int n = gradients(grads, x, wGateUp, h, dy, dz, dx, dGateUp, dDown, tokens, hidden, intermediate);
-  return n ? run<true, kStore>(grads, n, nullptr, dx ? workspace : nullptr, activation, status, s) : 0;
+  if (!n) return 0;
+  const size_t parts = purlin_ffn_workspace_bytes(tokens, hidden, intermediate, dx != nullptr, dGateUp != nullptr, dDown != nullptr);
+  return run<true, kStore>(grads, n, nullptr, parts && workspaceBytes >= parts ? workspace : nullptr, activation, status, s);
 }
 
 size_t purlin_ffn_workspace_bytes(int tokens, int hidden, int intermediate, int wantDx, int wantGateUp, int wantDown) {

@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4WideKernel(const __grid_co
 // ---- few rows: 128 rows of W are the rows of the MMA, the activations its columns, k split over a cluster ----
 // As in gemm_skinny.cuh: what bounds it is the read of W, every byte of which passes one SM once; the fp32 partial tiles are added in distributed
 // shared memory in ascending k order.
-constexpr int kFewThreads = skinny::kThreads, kFewTokens = 128, kWRows = 128;
+constexpr int kFewThreads = skinny::kThreads, kWRows = 128;
 
 struct FewParams {
   int N, K, tokens, cols;              // cols: columns of the MMA, tokens rounded up to 16
@@ -726,6 +726,10 @@ int launchFew(const void* aData, const void* aScales, const void* wData, const v
   return launched(cudaLaunchKernelEx(&cfg, kernel, maps, p)) ? 0 : 1;
 }
 
+// Rows of A up to which the kernel for few rows is taken (it has room for 128). The other one does not care how many of 256 there are, us, few rows 64 /
+// few rows 128 / the other: N, K 2048, 2048 5.7 / 7.2 / 6.3; 4096, 14336 13.5 / 19.8 / 17.7; 8192, 8192 11.6 / 15.7 / 12.4; 14336, 2048 gated 8.5 / 11.5 / 8.2.
+int fewRows(int N) { return N < 8192 ? 96 : 64; }
+
 int launchWide(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, bool swiglu, uint32_t* status, const Device& dev,
                cudaStream_t stream) {
   auto kernel = swiglu ? mx4WideKernel<true> : mx4WideKernel<false>;
@@ -786,6 +790,7 @@ size_t purlin_mx4_scale_bytes(int rows, int cols) { return rows > 0 && cols > 0 
 int purlin_mx4_quantize(const void* x, int dtype, void* data, void* scales, int rows, int cols, void* stream) {
   NvtxRange range("mx4Quantize", size_t(rows) * size_t(cols) / 2);
   if (!sizesFit(rows, cols)) return 1;
+  if (!x || !data || !scales) { setError("mx4: an operand is missing"); return 1; }
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales)) % 16) { setError("mx4: tensors must start on a 16-byte boundary"); return 1; }
   Device dev;
   if (!currentDevice(dev)) return 1;
@@ -801,6 +806,7 @@ int purlin_mx4_quantize(const void* x, int dtype, void* data, void* scales, int 
 int purlin_mx4_dequantize(const void* data, const void* scales, void* out, int dtype, int rows, int cols, void* stream) {
   NvtxRange range("mx4Dequantize", size_t(rows) * size_t(cols) / 2);
   if (!sizesFit(rows, cols)) return 1;
+  if (!data || !scales || !out) { setError("mx4: an operand is missing"); return 1; }
   if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales)) % 16) { setError("mx4: tensors must start on a 16-byte boundary"); return 1; }
   Device dev;
   if (!currentDevice(dev)) return 1;
@@ -821,7 +827,8 @@ int purlin_mx4_gemm(const void* aData, const void* aScales, const void* wData, c
   if (int64_t(M) * N / 4096 > INT32_MAX / 4 || scaleBytes(std::max(M, N), K) / 128 > size_t(INT32_MAX)) { setError("mx4: the product is too large"); return 1; }   // tile numbers, TMA coordinates
   Device dev;
   if (!currentDevice(dev)) return 1;
-  return M <= kFewTokens ? launchFew(aData, aScales, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream))
+  if (!aData || !aScales || !wData || !wScales || !C) { setError("mx4: an operand is missing"); return 1; }
+  return M <= fewRows(N) ? launchFew(aData, aScales, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream))
                          : launchWide(aData, aScales, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream));
 }
 

@@ -72,15 +72,14 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
         if (needs & 3) dz = at::empty({tokens, 2 * intermediate}, x.options());
         Tensor work;
         if (const size_t n = purlin_ffn_workspace_bytes(int(tokens), int(hidden), int(intermediate), int(needs & 1), int(needs & 2), int(needs & 4))) work = bytes(int64_t(n), x);
-        check(purlin_ffn_backward(x.data_ptr(), wGateUp.data_ptr(), wDown.data_ptr(), ptr(h), ptr(saved), dy.data_ptr(), ptr(dz), ptr(dx), ptr(dGateUp), ptr(dDown), ptr(work), int(tokens),
-                                  int(hidden), int(intermediate), int(ctx->saved_data["activation"].toInt()), nullptr, stream()));
+        check(purlin_ffn_backward(x.data_ptr(), wGateUp.data_ptr(), wDown.data_ptr(), ptr(h), ptr(saved), dy.data_ptr(), ptr(dz), ptr(dx), ptr(dGateUp), ptr(dDown), ptr(work),
+                                  work.defined() ? size_t(work.numel()) : 0, int(tokens), int(hidden), int(intermediate), int(ctx->saved_data["activation"].toInt()), nullptr, stream()));
       }
     }
     variable_list out{dx, dGateUp, dDown};
     if (again) {      // a graph through these gradients would be cut here without a word: whoever differentiates them is told
-      auto error = std::make_shared<torch::autograd::DelayedError>("gated_ffn is differentiable once", int64_t(out.size()));
-      for (Tensor& t : out) if (t.defined()) t.requires_grad_(true);
-      out = (*error)(std::move(out));
+      auto error = std::make_shared<torch::autograd::Error>("gated_ffn is differentiable once", torch::autograd::collect_next_edges(x, wGateUp, wDown, grads[0]));
+      for (Tensor& t : out) if (t.defined()) torch::autograd::create_gradient_edge(t, error);
     }
     out.emplace_back();
     return out;

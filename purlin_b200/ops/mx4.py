@@ -13,6 +13,7 @@ import torch
 from .. import _native
 
 EPI_STORE, EPI_SWIGLU = 0, 1
+MAX_ROWS = 2 ** 30
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -36,6 +37,8 @@ class Mx4Tensor:
             raise ValueError("data and scales must be contiguous CUDA tensors on one device")
         if (data.data_ptr() | scales.data_ptr()) % 16:
             raise ValueError("data and scales must start on a 16-byte boundary")
+        if data.shape[0] > MAX_ROWS:
+            raise ValueError("at most 2^30 rows")
         self.data, self.scales = data, scales
 
     @classmethod
@@ -74,6 +77,8 @@ def _check_dense(x: torch.Tensor):
         raise ValueError("operands must be contiguous CUDA tensors")
     if x.data_ptr() % 16:
         raise ValueError("operands must start on a 16-byte boundary")
+    if x.numel() // x.shape[-1] > MAX_ROWS:
+        raise ValueError("at most 2^30 rows")
 
 
 def quantize_mx4(x: torch.Tensor) -> Mx4Tensor:

@@ -134,3 +134,153 @@ def test_gated_product(m, i, k):
     from purlin_b200.ops.mx4 import mx4_gemm_swiglu, quantize_mx4
     a, w = quantize_mx4(_rand(m, k, 5)), quantize_mx4(_rand(2 * i, k, 6) * (4 * k ** -0.5))
     _check_product(mx4_gemm_swiglu(a, w), a, w, True)
+
+
+@pytest.mark.parametrize("m", [1, 63, 64, 65, 96, 97, 128, 129])
+@pytest.mark.parametrize("n", [8160, 8192])
+def test_both_kernels_at_their_border(m, n):
+    from purlin_b200.ops.mx4 import mx4_gemm, quantize_mx4
+    a, w = quantize_mx4(_rand(m, 288, 7, spread=2.0)), quantize_mx4(_rand(n, 288, 8, spread=2.0))
+    _check_product(mx4_gemm(a, w), a, w, False)
+
+
+@pytest.mark.parametrize("m", [2, 90, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_activations_quantised_in_the_call_and_given_outputs(m, dtype):
+    from purlin_b200.ops.mx4 import mx4_gemm, mx4_gemm_swiglu, quantize_mx4
+    x, w = _rand(m, 224, 9, dtype), quantize_mx4(_rand(544, 224, 10))
+    q = quantize_mx4(x)
+    for f, cols in ((mx4_gemm, 544), (mx4_gemm_swiglu, 272)):
+        want = f(q, w)
+        assert torch.equal(f(x, w), want)
+        out = torch.full((m + 2, cols), 7.0, dtype=torch.bfloat16, device="cuda")
+        assert f(x, w, out[1:-1]) .data_ptr() == out[1:-1].data_ptr()
+        assert torch.equal(out[1:-1], want) and (out[0] == 7).all() and (out[-1] == 7).all()
+        assert torch.equal(f(q, w, out[1:-1]), want)
+        assert torch.equal(f(x.view(1, m, 224), w), want.view(1, m, cols))
+        assert f(x[0], w).shape == (cols,)
+        assert f(x[:0], w).shape == (0, cols) and f(x[:0].view(3, 0, 224), w).shape == (3, 0, cols)
+    assert quantize_mx4(x[:0]).shape == (0, 224) and quantize_mx4(x[:0]).dequantize().shape == (0, 224)
+
+
+@pytest.mark.parametrize("m", [3, 70, 200])
+def test_nans_stay_in_their_rows_and_columns(m):
+    from purlin_b200.ops.mx4 import mx4_gemm, quantize_mx4
+    x, w = _rand(m, 288, 11), _rand(264, 288, 12)
+    clean = mx4_gemm(quantize_mx4(x), quantize_mx4(w))
+    bad_x, bad_w = x.clone(), w.clone()
+    bad_x[1, 280], bad_w[130, 3] = float("nan"), float("inf")
+    got = mx4_gemm(quantize_mx4(bad_x), quantize_mx4(bad_w))
+    rows, cols = torch.arange(m) != 1, torch.arange(264) != 130
+    assert got[1].isnan().all() and got[:, 130].isnan().all()
+    assert torch.equal(got[rows][:, cols], clean[rows][:, cols])
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 264, 544), (300, 520, 544)])
+def test_scales_at_the_ends_of_their_range(m, n, k):
+    # powers of two from 2^-127 to 2^125 on one side and their inverses on the other: products and sums that fp32 holds exactly
+    from purlin_b200.ops.mx4 import mx4_gemm, quantize_mx4
+    g = torch.Generator(device="cuda").manual_seed(13)
+    e = torch.tensor([-100.0, -60.0, 0.0, 60.0, 100.0], device="cuda")[torch.randint(0, 5, (k // 32,), generator=g, device="cuda")]
+    power = torch.exp2(e).repeat_interleave(32)
+    a = torch.randint(-4, 5, (m, k), generator=g, device="cuda").float() * power
+    w = torch.randint(-1, 2, (n, k), generator=g, device="cuda").float() / power
+    a[:, ::32], w[:, ::32] = 4 * power[::32], 4 / power[::32]          # so that every block's largest magnitude is 4: whole numbers are exact
+    got = mx4_gemm(quantize_mx4(a), quantize_mx4(w))
+    ref = quantize_mx4(a).dequantize(torch.float32).double() @ quantize_mx4(w).dequantize(torch.float32).double().t()
+    assert torch.equal(got.double(), ref.to(torch.bfloat16).double())
+
+
+def test_bits_do_not_change_from_call_to_call():
+    from purlin_b200.ops.mx4 import mx4_gemm_swiglu, quantize_mx4
+    w = quantize_mx4(_rand(2048, 4096, 14))
+    for m in (1, 50, 500):
+        x = _rand(m, 4096, 15)
+        first = mx4_gemm_swiglu(x, w)
+        for _ in range(4):
+            assert torch.equal(mx4_gemm_swiglu(x, w), first)
+
+
+def test_on_a_stream_of_its_own_and_in_graphs():
+    from purlin_b200.ops.mx4 import mx4_gemm, mx4_gemm_swiglu, quantize_mx4
+    wg, wd = quantize_mx4(_rand(1024, 288, 16) * 0.1), quantize_mx4(_rand(288, 512, 17) * 0.1)
+
+    def block(x):
+        return mx4_gemm(mx4_gemm_swiglu(x, wg), wd)
+
+    xs = {m: _rand(m, 288, 18 + m) for m in (1, 300)}
+    want = {m: block(x) for m, x in xs.items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = {m: block(x) for m, x in xs.items()}
+    side.synchronize()
+    assert all(torch.equal(got[m], want[m]) for m in xs)
+    graphs = {}
+    for m, x in xs.items():
+        static, g = x.clone(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = block(static)
+        graphs[m] = (g, static, y)
+    for seed in (1, 2):
+        for m, (g, static, y) in graphs.items():
+            static.copy_(_rand(m, 288, seed))
+            g.replay()
+            assert torch.equal(y, block(_rand(m, 288, seed)))
+
+
+def test_a_tensor_of_more_than_4_gib():
+    from purlin_b200.ops.mx4 import quantize_mx4
+    rows, cols = 140003, 16416                                # 4.6 GB of bf16, codes of more than 2^31 values
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    for r in range(0, rows, 20000):
+        x[r:r + 20000] = _rand(min(20000, rows - r), cols, r)
+    q = quantize_mx4(x)
+    v = q.dequantize()
+    scales = q.scale_matrix()
+    for r in (0, 65535, 130999, rows - 40):
+        part = quantize_mx4(x[r:r + 40].clone())
+        assert torch.equal(q.data[r:r + 40], part.data) and torch.equal(v[r:r + 40], part.dequantize()) and torch.equal(scales[r:r + 40], part.scale_matrix())
+
+
+def test_refusals_of_tensors_on_the_gpu():
+    from purlin_b200.ops.gated_ffn import gated_ffn
+    from purlin_b200.ops.mx4 import Mx4Tensor, mx4_gemm, mx4_gemm_swiglu, quantize_mx4
+    x, w = _rand(4, 64, 1), quantize_mx4(_rand(48, 64, 2))
+    flat = torch.zeros(4 * 64 + 8, dtype=torch.bfloat16, device="cuda")
+    for bad in (x.t().contiguous().t(), x[:, ::2], flat[1:257].view(4, 64)):
+        for f in (quantize_mx4, lambda v: mx4_gemm(v, w)):
+            with pytest.raises(ValueError):
+                f(bad)
+    with pytest.raises(TypeError):
+        mx4_gemm(x, x)
+    with pytest.raises(TypeError):
+        quantize_mx4(x.long())
+    with pytest.raises(ValueError):
+        mx4_gemm(x[:, :32].contiguous(), w)
+    with pytest.raises(ValueError):
+        mx4_gemm_swiglu(x, w)                                  # 48 rows are no whole groups of gate and up
+    with pytest.raises(ValueError):
+        mx4_gemm(x, quantize_mx4(_rand(4, 64, 2)))
+    with pytest.raises(TypeError):
+        mx4_gemm(x, w, torch.empty(4, 48, device="cuda"))
+    for out in (torch.empty(4, 40, device="cuda", dtype=torch.bfloat16), torch.empty(48, 4, device="cuda", dtype=torch.bfloat16).t()):
+        with pytest.raises(ValueError):
+            mx4_gemm(x, w, out)
+    with pytest.raises(ValueError):
+        Mx4Tensor(w.data, w.scales[:-1])
+    with pytest.raises(ValueError):
+        Mx4Tensor(w.data.t(), w.scales)
+    with pytest.raises(TypeError):
+        Mx4Tensor(w.data.int(), w.scales)
+    with pytest.raises(TypeError):
+        w.dequantize(torch.float16)
+    same = Mx4Tensor(w.data.clone(), w.scales.clone())          # what a checkpoint gives back
+    assert torch.equal(mx4_gemm(x, same), mx4_gemm(x, w))
+    g = torch.zeros(64, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        gated_ffn(x.t().contiguous().t(), g, torch.zeros(64, 32, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ValueError):
+        gated_ffn(flat[1:257].view(4, 64), g, torch.zeros(64, 32, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ValueError):
+        gated_ffn(x.cpu(), g, torch.zeros(64, 32, dtype=torch.bfloat16, device="cuda"))
