@@ -701,10 +701,25 @@ int launchAs(Params& p, int groups, const Shape& s, const Device& dev, cudaStrea
 
 // C[M, N] (or the gated forms) = sum over k of A(m, k) B(n, k). A is [M, K] row-major, or [K, M] with aMn; B is [N, K], or [K, N] with B_MN.
 struct Product { const void *A, *B; void* C; int M, N, K; bool aMn; };
+// A function of the sizes (and of the number of SMs): each thread keeps those of its recent sizes, some microseconds of host time.
 Shape shapeOf(const Product* products, int n, const Device& dev, int epi, bool mayCut) {
+  struct Known { Sizes z[kMaxGroups]; int n, sms, epi; bool mayCut; Shape s; };
+  static thread_local Known recent[64] = {};
   Sizes z[kMaxGroups] = {};
-  for (int i = 0; i < n; ++i) z[i] = Sizes{products[i].M, products[i].N, products[i].K};
-  return chooseShape(z, n, dev.sms, epi, mayCut);
+  uint32_t hash = uint32_t(n * 8 + epi * 2 + int(mayCut)) * 2654435761u;
+  for (int i = 0; i < n; ++i) {
+    z[i] = Sizes{products[i].M, products[i].N, products[i].K};
+    hash = (hash ^ uint32_t(z[i].M)) * 2246822519u + uint32_t(z[i].N) * 3266489917u + uint32_t(z[i].K);
+  }
+  Known& k = recent[hash >> 26];
+  bool same = k.n == n && k.sms == dev.sms && k.epi == epi && k.mayCut == mayCut;
+  for (int i = 0; i < n; ++i) same = same && k.z[i].M == z[i].M && k.z[i].N == z[i].N && k.z[i].K == z[i].K;
+  if (!same) {
+    k.s = chooseShape(z, n, dev.sms, epi, mayCut);
+    for (int i = 0; i < n; ++i) k.z[i] = z[i];
+    k.n = n; k.sms = dev.sms; k.epi = epi; k.mayCut = mayCut;
+  }
+  return k.s;
 }
 // `partial`: room for the parts of the first product's k, or null where it is not to be cut
 template <bool B_MN, int EPI>
