@@ -27,9 +27,11 @@ int purlin_mx4_dequantize(const void* data, const void* scales, void* out, int d
  * alternate 16 of gate and 16 of up, N a multiple of 32, C is [M, N / 2]). N a multiple of 8. status: as in purlin_gemm_bf16. */
 int purlin_mx4_gemm(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue,
                     uint32_t* status, void* stream);
-/* The same with activations x [M, K] of `dtype`, which are quantised into aData and aScales (workspace) first. */
-int purlin_mx4_linear(const void* x, int dtype, void* aData, void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K,
-                      int epilogue, uint32_t* status, void* stream);
+/* The same with activations x [M, K] of `dtype`, quantised by the way: a few tokens inside the product, more into the workspace first, which has
+ * purlin_mx4_workspace_bytes() (none: it may be NULL). */
+size_t purlin_mx4_workspace_bytes(int dtype, int M, int K);
+int purlin_mx4_linear(const void* x, int dtype, void* workspace, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue,
+                      uint32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -36,7 +36,8 @@ constexpr int kScaleRows = 128, kScaleCols = 128, kScaleBytes = 512;
 // Four lanes have the 32 values of a block (8 each, 16 bytes of bf16 or fp16), a warp 256 columns, and a step of a warp is four of those side by
 // side in one row. The scale needs the exponent of the largest magnitude only, a byte, so the four blocks of a lane travel through the
 // shuffles in one word, and four more shuffles' worth of bytes become the words of the scales' layout in two. With one shuffle chain per block and
-// 64-bit index arithmetic the instructions, not the memory, were the bound (8192 x 8192 there and back 104 us).
+// 64-bit index arithmetic the instructions, not the memory, were the bound. One B200, 8192 x 8192 bf16: 28.6 us, 5.9 TB/s (0.91 of a copy);
+// the way back 33 us, 5.1 TB/s; there and back with one chain per block 104 us.
 constexpr int kVec = 8, kWarpCols = 32 * kVec, kQuantThreads = 256, kUnroll = 4, kStepCols = kUnroll * kWarpCols;
 
 PURLIN_D uint4 ldOnce(const void* p) {
@@ -84,6 +85,20 @@ template <int TYPE> PURLIN_D void toFloats(const Raw<TYPE>& r, float (&f)[kVec])
   }
 }
 
+// eight values times a power of two, rounded to the nearest of the format (ties to the even code), the first in the lowest four bits
+PURLIN_D uint32_t packCodes(const float (&f)[kVec], float inverse) {
+  float2 v[kVec / 2];
+#pragma unroll
+  for (int i = 0; i < kVec / 2; ++i) v[i] = __fmul2_rn(make_float2(f[2 * i], f[2 * i + 1]), make_float2(inverse, inverse));
+  uint32_t codes;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(codes) : "f"(v[0].x), "f"(v[0].y), "f"(v[1].x), "f"(v[1].y), "f"(v[2].x), "f"(v[2].y), "f"(v[3].x), "f"(v[3].y));
+  return codes;
+}
+
 PURLIN_D size_t scaleOffset(int row, int col, int colBlocks) {       // of the scale of this row's block that begins at `col`
   return (size_t(row / kScaleRows) * size_t(colBlocks) + size_t(col / kScaleCols)) * kScaleBytes + size_t(row % 32) * 16 + size_t(row / 32 % 4) * 4 + size_t(col / kBlock % 4);
 }
@@ -121,10 +136,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantizeKernel(const unsigned c
       const float inverse = __uint_as_float((254u - scale) << 23);       // (of a scale of 255 not used)
       float f[kVec];
       toFloats<TYPE>(raw[u], f);
-      uint32_t codes = 0;
-#pragma unroll
-      for (int e = 0; e < kVec; e += 2)
-        codes |= uint32_t(__nv_cvt_float2_to_fp4x2(make_float2(f[e] * inverse, f[e + 1] * inverse), __NV_E2M1, cudaRoundNearest)) << (4 * e);
+      uint32_t codes = packCodes(f, inverse);
       if (scale == 255u) codes = 0;
       if (row < rows && col + u * kWarpCols < cols) *reinterpret_cast<uint32_t*>(data + (at + size_t(u * kWarpCols)) / 2) = codes;
     }
@@ -452,7 +464,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4WideKernel(const __grid_co
 // ---- few rows: 128 rows of W are the rows of the MMA, the activations its columns, k split over a cluster ----
 // As in gemm_skinny.cuh: what bounds it is the read of W, every byte of which passes one SM once; the fp32 partial tiles are added in distributed
 // shared memory in ascending k order.
+// DENSE: the activations come as bf16, and the four warps that wait for the sums quantise them in the meantime, every CTA its own k range of
+// them, straight into the stages: one launch instead of two for a handful of tokens (one B200, us, two launches / one: 1 x 2048 x 2048 5.5 / 4.3, 1 x 7168 x 8192 8.9 / 7.6,
+// 4 x 57344 x 8192 43.6 / 42.0; with two tokens to a warp 50.8, so up to four tokens).
 constexpr int kFewThreads = skinny::kThreads, kWRows = 128;
+constexpr int kDenseTokens = 4, kDenseBytes = kDenseTokens * kBK * 2;      // a token to a warp; of bf16 activations in a stage
 
 struct FewParams {
   int N, K, tokens, cols;              // cols: columns of the MMA, tokens rounded up to 16
@@ -462,20 +478,49 @@ struct FewParams {
   uint32_t* status;
   uint64_t timeoutNs;
 };
-PURLIN_HD int fewStageBytes(int cols) { return kABytes + cols * 128 + 2 * kScaleStage; }     // [W][X][scales W][scales X]
+PURLIN_HD int fewStageBytes(int cols, bool dense) { return kABytes + cols * 128 + 2 * kScaleStage + (dense ? kDenseBytes : 0); }     // [W][X][scales W][scales X][bf16 X]
 
-template <bool SWIGLU>
+// Token w, 256 columns to a stage: from the bf16 values that TMA has brought into the stage to codes in the swizzled tile and scales in their blocks.
+// (Tokens that there are not are zeros.) Plain loads, however early, would be waited for by every fence to the tensor core's proxy.
+PURLIN_D bool quantiseStages(const FewParams& p, uint32_t base, uint32_t stageBytes, uint32_t fullBars, uint32_t denseBars, int w, int lane, int count, volatile int* abortWord) {
+  uint32_t st = 0, ph = 0;
+  for (int i = 0; i < count; ++i) {
+    if (!waitAll(denseBars + 8u * st, ph, abortWord, p.timeoutNs)) { if (lane == 0) skinny::recordTimeout(p.status, 7, w, i); return false; }
+    const uint32_t sX = base + st * stageBytes + kABytes, sS = sX + uint32_t(p.cols * 128) + kScaleStage, sD = sS + kScaleStage;
+    Raw<PURLIN_MX4_BF16> raw;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(raw.v[0].x), "=r"(raw.v[0].y), "=r"(raw.v[0].z), "=r"(raw.v[0].w) : "r"(sD + uint32_t(w) * (kBK * 2) + uint32_t(lane) * 16u) : "memory");
+    uint32_t peak = peakExponent<PURLIN_MX4_BF16>(raw);
+    peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+    peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+    const uint32_t scale = peak == 255u ? 255u : peak > 2u ? peak - 2u : 0u;
+    float f[kVec];
+    toFloats<PURLIN_MX4_BF16>(raw, f);
+    const uint32_t codes = scale == 255u ? 0u : packCodes(f, __uint_as_float((254u - scale) << 23));
+    uint32_t word = scale << (8 * (lane / 4 % 4));
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(sX + uint32_t(w) * 128u + (uint32_t(lane / 4) ^ uint32_t(w & 7)) * 16u + uint32_t(lane % 4) * 4u), "r"(codes) : "memory");
+    if (lane % 16 == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sS + uint32_t(lane / 16) * kScaleBytes + uint32_t(w) * 16u), "r"(word) : "memory");
+    tc::fenceProxyAsyncShared();
+    __syncwarp();
+    if (lane == 0) tc::mbarArrive(fullBars + 8u * st);
+    if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
+  }
+  return true;
+}
+
+template <bool SWIGLU, bool DENSE>
 __global__ void __launch_bounds__(kFewThreads, 2) mx4FewKernel(const __grid_constant__ Maps maps, const __grid_constant__ FewParams p) {
   extern __shared__ unsigned char smemRaw[];
   const uint32_t rawAddr = tc::smemAddr(smemRaw);
   const uint32_t base = (rawAddr + 1023u) & ~1023u;
   unsigned char* smem = smemRaw + (base - rawAddr);
-  const uint32_t stageBytes = uint32_t(fewStageBytes(p.cols));
+  const uint32_t stageBytes = uint32_t(fewStageBytes(p.cols, DENSE));
   const uint32_t barBase = base + uint32_t(p.stages) * stageBytes;
   auto fullBar = [&](uint32_t s) { return barBase + 8u * s; };
   auto emptyBar = [&](uint32_t s) { return barBase + 8u * (uint32_t(p.stages) + s); };
-  const uint32_t accFull = barBase + 8u * (2u * uint32_t(p.stages)), mmasDone = accFull + 8u;
-  uint32_t* words = reinterpret_cast<uint32_t*>(smem + size_t(p.stages) * stageBytes + 8 * (2 * p.stages + 2));
+  const uint32_t accFull = barBase + 8u * (2u * uint32_t(p.stages)), mmasDone = accFull + 8u, denseBars = mmasDone + 8u;      // denseBars: bf16 activations of a stage
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem + size_t(p.stages) * stageBytes + 8 * (3 * p.stages + 2));
   volatile uint32_t* tmemBaseWord = words;
   volatile int* abortWord = reinterpret_cast<volatile int*>(words + 1);
 
@@ -486,7 +531,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) mx4FewKernel(const __grid_cons
   const int tile = int(blockIdx.x / split);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) { tc::mbarInit(fullBar(s), 1); tc::mbarInit(emptyBar(s), 1); }
+    for (int s = 0; s < p.stages; ++s) { tc::mbarInit(fullBar(s), DENSE ? 5 : 1); tc::mbarInit(emptyBar(s), 1); tc::mbarInit(denseBars + 8u * uint32_t(s), 1); }      // (the four quantising warps arrive too)
     tc::mbarInit(accFull, 1);
     tc::mbarInit(mmasDone, 1);
     *abortWord = 0;
@@ -518,11 +563,16 @@ __global__ void __launch_bounds__(kFewThreads, 2) mx4FewKernel(const __grid_cons
       if (!ok) { if (elected) skinny::recordTimeout(p.status, 1, tile, kb); break; }
       const uint32_t sW = base + st * stageBytes, sX = sW + kABytes, sS = sX + uint32_t(p.cols * 128);
       if (elected) {
-        tc::mbarExpectTx(fullBar(st), stageBytes);
+        tc::mbarExpectTx(fullBar(st), DENSE ? uint32_t(kABytes + kScaleStage) : stageBytes);
         tc::tmaLoad2d(sW, &maps.a, kb * 128, tile * kWRows, fullBar(st));
         loadScalesHere(sS, &maps.sa, 8 * kb, tile, fullBar(st));
-        tc::tmaLoad2d(sX, &maps.b, kb * 128, 0, fullBar(st));
-        loadScalesHere(sS + kScaleStage, &maps.sb, 8 * kb, 0, fullBar(st));
+        if constexpr (DENSE) {
+          tc::mbarExpectTx(denseBars + 8u * st, kDenseBytes);
+          tc::tmaLoad2d(sS + 2 * kScaleStage, &maps.b, kb * kBK, 0, denseBars + 8u * st);
+        } else {
+          tc::tmaLoad2d(sX, &maps.b, kb * 128, 0, fullBar(st));
+          loadScalesHere(sS + kScaleStage, &maps.sb, 8 * kb, 0, fullBar(st));
+        }
       }
       __syncwarp();
       if (++st == uint32_t(p.stages)) { st = 0; ph ^= 1; }
@@ -555,8 +605,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) mx4FewKernel(const __grid_cons
   } else {
     // ---- this CTA's partial tile: TMEM (lane = row of W, column = token) -> shared memory [token][row of W] ----
     const int quarter = warp & 3;
-    ok = tc::mbarWait(accFull, 0, abortWord, p.timeoutNs);
-    ok = __all_sync(0xffffffffu, ok);
+    if constexpr (DENSE) ok = quantiseStages(p, base, stageBytes, barBase, denseBars, warp - 2, lane, kEnd - kBegin, abortWord);
+    if (ok) ok = waitAll(accFull, 0, abortWord, p.timeoutNs);
     if (!ok && lane == 0) skinny::recordTimeout(p.status, 5, tile, 0);
     if (ok) {
       // every load has landed and every MMA has read its stage, so the stages' memory is free
@@ -603,8 +653,13 @@ __global__ void __launch_bounds__(kFewThreads, 2) mx4FewKernel(const __grid_cons
   }
   tc::clusterSync();                    // nobody leaves behind a partial tile that a peer still reads
   if (*abortWord) {
-    if (warp == 0 && lane == 0) for (uint32_t s = 0; s < uint32_t(p.stages); ++s) tc::mbarDrain(fullBar(s), s < st ? ph : ph ^ 1);
-    if (warp == 1 && lane == 0) { tc::mmaCommit(mmasDone); tc::mbarDrain(mmasDone, 0); }
+    if (DENSE) tc::landingPause();      // (a stage that was not quantised never completes)
+    else if (warp == 0 && lane == 0) for (uint32_t s = 0; s < uint32_t(p.stages); ++s) tc::mbarDrain(fullBar(s), s < st ? ph : ph ^ 1);
+    if (warp == 1) {                    // (a commit counts what its own thread has issued)
+      const uint32_t elected = electOne();
+      commit<1>(elected, mmasDone);
+      if (elected) tc::mbarDrain(mmasDone, 0);
+    }
     __syncwarp();
   }
   tc::fenceBeforeThreadSync();
@@ -683,6 +738,18 @@ bool outputMap(CUtensorMap* map, void* ptr, uint64_t rows, uint64_t cols) {
   return true;
 }
 
+// bf16 activations, a few rows x 256 columns to a box, as they lie
+bool denseMap(CUtensorMap* map, const void* ptr, int rows, int cols) {
+  const TensorMapEncodeFn fn = tensorMapEncodeFn();
+  if (!fn) { setError("cuTensorMapEncodeTiled is not available from this driver"); return false; }
+  const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)}, strides[1] = {cuuint64_t(cols) * 2};
+  const cuuint32_t box[2] = {kBK, kDenseTokens}, elem[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { setError("cuTensorMapEncodeTiled failed with code " + std::to_string(int(r))); return false; }
+  return true;
+}
+
 size_t scaleBytes(int rows, int cols) { return size_t((rows + kScaleRows - 1) / kScaleRows) * size_t((cols + kScaleCols - 1) / kScaleCols) * kScaleBytes; }
 
 bool optIn(const void* kernel, bool& done) {
@@ -693,7 +760,7 @@ bool optIn(const void* kernel, bool& done) {
   return true;
 }
 
-int launchFew(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, bool swiglu, uint32_t* status, const Device& dev,
+int launchFew(const void* x, const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, bool swiglu, uint32_t* status, const Device& dev,
               cudaStream_t stream) {
   const int outCols = swiglu ? N / 2 : N;
   if (reinterpret_cast<uintptr_t>(C) % 16) { setError("TMA operands need 16-byte aligned base and row pitch"); return 1; }
@@ -707,24 +774,35 @@ int launchFew(const void* aData, const void* aScales, const void* wData, const v
   const int used = (p.cols + 31) / 32 * 32 + 32;
   p.tmemCols = used <= 64 ? 64 : used <= 128 ? 128 : 256;
   // the partial tile [tokens][128] in fp32 takes the place of the stages
-  const int room = 113 * 1024 - 1024 - 256, stage = fewStageBytes(p.cols);
+  const int room = 113 * 1024 - 1024 - 256, stage = fewStageBytes(p.cols, x != nullptr);
   p.stages = std::max(std::min({room / stage, 8, std::max((kBlocks + split - 1) / split, 2)}), (M * kWRows * 4 + stage - 1) / stage);
   p.ahead = std::min(p.stages, 4);
   Maps maps{};
-  if (!makeTensorMap(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, wData, uint64_t(N), uint64_t(K) / 2, uint64_t(K) / 2, kWRows) ||
-      !makeTensorMap(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, aData, uint64_t(M), uint64_t(K) / 2, uint64_t(K) / 2, uint32_t(p.cols)) ||
-      !scaleMap(&maps.sa, wScales, N, K, 1) || !scaleMap(&maps.sb, aScales, M, K, 1)) return 1;
-  auto kernel = swiglu ? mx4FewKernel<true> : mx4FewKernel<false>;
-  static bool done[64][2] = {};
-  if (!optIn(reinterpret_cast<const void*>(kernel), done[dev.index][swiglu])) return 1;
+  if (!makeTensorMap(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, wData, uint64_t(N), uint64_t(K) / 2, uint64_t(K) / 2, kWRows) || !scaleMap(&maps.sa, wScales, N, K, 1)) return 1;
+  if (x ? !denseMap(&maps.b, x, M, K)
+        : !makeTensorMap(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, aData, uint64_t(M), uint64_t(K) / 2, uint64_t(K) / 2, uint32_t(p.cols)) || !scaleMap(&maps.sb, aScales, M, K, 1)) return 1;
+  auto kernel = x ? (swiglu ? mx4FewKernel<true, true> : mx4FewKernel<false, true>) : swiglu ? mx4FewKernel<true, false> : mx4FewKernel<false, false>;
+  static bool done[64][4] = {};
+  if (!optIn(reinterpret_cast<const void*>(kernel), done[dev.index][(x ? 2 : 0) + swiglu])) return 1;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = unsigned(split); attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(unsigned(tiles) * unsigned(split)); cfg.blockDim = dim3(kFewThreads); cfg.stream = stream;
-  cfg.dynamicSmemBytes = size_t(p.stages) * size_t(stage) + 256 + 1024; cfg.attrs = attr; cfg.numAttrs = 2;
+  cfg.dynamicSmemBytes = size_t(p.stages) * size_t(stage) + kBarrierBytes + 1024; cfg.attrs = attr; cfg.numAttrs = 2;
   return launched(cudaLaunchKernelEx(&cfg, kernel, maps, p)) ? 0 : 1;
 }
+
+bool productFits(int M, int N, int K, int epilogue) {
+  if (!sizesFit(M, K) || !sizesFit(N, K)) return false;
+  if (epilogue != PURLIN_EPI_STORE && epilogue != PURLIN_EPI_SWIGLU) { setError("unknown epilogue"); return false; }
+  const bool swiglu = epilogue == PURLIN_EPI_SWIGLU;
+  if (N % (swiglu ? 32 : 8)) { setError(swiglu ? "the SwiGLU epilogue needs N to be a multiple of 32" : "mx4: N must be a multiple of 8"); return false; }
+  if (int64_t(M) * N / 4096 > INT32_MAX / 4 || scaleBytes(std::max(M, N), K) / 128 > size_t(INT32_MAX)) { setError("mx4: the product is too large"); return false; }   // tile numbers, TMA coordinates
+  return true;
+}
+// whether the product quantises its activations itself
+bool quantisedInside(int dtype, int M) { return dtype == PURLIN_MX4_BF16 && M <= kDenseTokens; }
 
 // Rows of A up to which the kernel for few rows is taken (it has room for 128). The other one does not care how many of 256 there are, us, few rows 64 /
 // few rows 128 / the other: N, K 2048, 2048 5.7 / 7.2 / 6.3; 4096, 14336 13.5 / 19.8 / 17.7; 8192, 8192 11.6 / 15.7 / 12.4; 14336, 2048 gated 8.5 / 11.5 / 8.2.
@@ -821,20 +899,34 @@ int purlin_mx4_dequantize(const void* data, const void* scales, void* out, int d
 int purlin_mx4_gemm(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue, uint32_t* status, void* stream) {
   const bool swiglu = epilogue == PURLIN_EPI_SWIGLU;
   NvtxRange range(swiglu ? "mx4GemmSwiglu" : "mx4Gemm", size_t(M) * size_t(N) * 2);
-  if (!sizesFit(M, K) || !sizesFit(N, K)) return 1;
-  if (epilogue != PURLIN_EPI_STORE && !swiglu) { setError("unknown epilogue"); return 1; }
-  if (N % (swiglu ? 32 : 8)) { setError(swiglu ? "the SwiGLU epilogue needs N to be a multiple of 32" : "mx4: N must be a multiple of 8"); return 1; }
-  if (int64_t(M) * N / 4096 > INT32_MAX / 4 || scaleBytes(std::max(M, N), K) / 128 > size_t(INT32_MAX)) { setError("mx4: the product is too large"); return 1; }   // tile numbers, TMA coordinates
   Device dev;
-  if (!currentDevice(dev)) return 1;
+  if (!productFits(M, N, K, epilogue)) return 1;
   if (!aData || !aScales || !wData || !wScales || !C) { setError("mx4: an operand is missing"); return 1; }
-  return M <= fewRows(N) ? launchFew(aData, aScales, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream))
+  if (!currentDevice(dev)) return 1;
+  return M <= fewRows(N) ? launchFew(nullptr, aData, aScales, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream))
                          : launchWide(aData, aScales, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream));
 }
 
-int purlin_mx4_linear(const void* x, int dtype, void* aData, void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue, uint32_t* status, void* stream) {
-  const int rc = purlin_mx4_quantize(x, dtype, aData, aScales, M, K, stream);
-  return rc ? rc : purlin_mx4_gemm(aData, aScales, wData, wScales, C, M, N, K, epilogue, status, stream);
+size_t purlin_mx4_workspace_bytes(int dtype, int M, int K) {
+  return M <= 0 || K <= 0 || quantisedInside(dtype, M) ? 0 : size_t(M) * size_t(K) / 2 + scaleBytes(M, K);
+}
+
+int purlin_mx4_linear(const void* x, int dtype, void* workspace, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue, uint32_t* status, void* stream) {
+  if (!productFits(M, N, K, epilogue)) return 1;
+  if (quantisedInside(dtype, M)) {
+    const bool swiglu = epilogue == PURLIN_EPI_SWIGLU;
+    NvtxRange range(swiglu ? "mx4LinearSwiglu" : "mx4Linear", size_t(M) * size_t(N) * 2);
+    Device dev;
+    if (!x || !wData || !wScales || !C) { setError("mx4: an operand is missing"); return 1; }
+    if (reinterpret_cast<uintptr_t>(x) % 16) { setError("mx4: tensors must start on a 16-byte boundary"); return 1; }
+    if (!currentDevice(dev)) return 1;
+    return launchFew(x, nullptr, nullptr, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream));
+  }
+  unsigned char* data = static_cast<unsigned char*>(workspace);
+  if (!data) { setError("mx4: an operand is missing"); return 1; }
+  unsigned char* scales = data + size_t(M) * size_t(K) / 2;       // (a row is a multiple of 16 bytes)
+  const int rc = purlin_mx4_quantize(x, dtype, data, scales, M, K, stream);
+  return rc ? rc : purlin_mx4_gemm(data, scales, wData, wScales, C, M, N, K, epilogue, status, stream);
 }
 
 }  // extern "C"

@@ -113,10 +113,9 @@ void product(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales
   if (aScales) {
     check(purlin_mx4_gemm(a.data_ptr(), aScales->data_ptr(), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), int(rows), int(n), int(k), int(epilogue), nullptr, stream()));
   } else {
-    const int64_t values = rows * k / 2;      // (a row is a multiple of 16 bytes)
-    const Tensor work = bytes(values + int64_t(purlin_mx4_scale_bytes(int(rows), int(k))), wData);
-    unsigned char* at = static_cast<unsigned char*>(work.data_ptr());
-    check(purlin_mx4_linear(a.data_ptr(), int(type), at, at + values, wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), int(rows), int(n), int(k), int(epilogue), nullptr, stream()));
+    Tensor work;
+    if (const size_t size = purlin_mx4_workspace_bytes(int(type), int(rows), int(k))) work = bytes(int64_t(size), wData);
+    check(purlin_mx4_linear(a.data_ptr(), int(type), ptr(work), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), int(rows), int(n), int(k), int(epilogue), nullptr, stream()));
   }
 }
 Tensor newProduct(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales, const Tensor& wData, const Tensor& wScales, std::vector<int64_t> shape, int64_t rows,

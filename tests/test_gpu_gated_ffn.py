@@ -322,3 +322,12 @@ def test_a_training_step_through_the_model_then_4_bits():
         hq = quantize_mx4(mine).dequantize(torch.float32).double()
         ref, m = hq @ w_down.t(), hq.abs() @ w_down.abs().t()
         assert ((got.double() - ref).abs() <= STEP * ref.abs() + 2.0 ** -16 * m + 1e-30).all()
+
+
+def test_example():
+    import pathlib
+    import subprocess
+    import sys
+    example = pathlib.Path(__file__).resolve().parent.parent / "examples" / "gated_mlp.py"
+    done = subprocess.run([sys.executable, str(example), "200", "512", "1024"], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip().endswith("ok"), done.stdout + done.stderr      # it checks its own gradients

@@ -121,7 +121,7 @@ def test_few_rows(m, n, k):
     _check_product(mx4_gemm(a, w), a, w, False)
 
 
-@pytest.mark.parametrize("m,n,k", [(129, 8, 32), (129, 264, 96), (256, 256, 256), (257, 128, 64), (300, 520, 544), (511, 1000, 288), (1000, 1024, 1120), (513, 14336, 256), (2049, 4104, 96),
+@pytest.mark.parametrize("m,n,k", [(129, 8, 32), (129, 264, 96), (256, 256, 256), (257, 128, 64), (300, 520, 544), (511, 1000, 288), (1000, 1024, 1120), (513, 14336, 256), (2049, 4104, 96), (200, 14208, 256), (500, 7104, 288),
                                     (4096, 2048, 2048)])
 def test_many_rows(m, n, k):
     from purlin_b200.ops.mx4 import mx4_gemm, quantize_mx4
@@ -129,7 +129,7 @@ def test_many_rows(m, n, k):
     _check_product(mx4_gemm(a, w), a, w, False)
 
 
-@pytest.mark.parametrize("m,i,k", [(1, 16, 32), (1, 3584, 1024), (7, 80, 96), (100, 528, 544), (128, 1024, 512), (129, 16, 64), (300, 528, 224), (1000, 1040, 512), (777, 7168, 256)])
+@pytest.mark.parametrize("m,i,k", [(1, 16, 32), (1, 3584, 1024), (7, 80, 96), (100, 528, 544), (128, 1024, 512), (129, 16, 64), (300, 528, 224), (1000, 1040, 512), (777, 7168, 256), (200, 7104, 256)])
 def test_gated_product(m, i, k):
     from purlin_b200.ops.mx4 import mx4_gemm_swiglu, quantize_mx4
     a, w = quantize_mx4(_rand(m, k, 5)), quantize_mx4(_rand(2 * i, k, 6) * (4 * k ** -0.5))
@@ -284,3 +284,21 @@ def test_refusals_of_tensors_on_the_gpu():
         gated_ffn(flat[1:257].view(4, 64), g, torch.zeros(64, 32, dtype=torch.bfloat16, device="cuda"))
     with pytest.raises(ValueError):
         gated_ffn(x.cpu(), g, torch.zeros(64, 32, dtype=torch.bfloat16, device="cuda"))
+
+
+@pytest.mark.parametrize("m", [1, 3, 4, 5, 8, 15, 16, 17])
+@pytest.mark.parametrize("n,k", [(64, 32), (264, 96), (160, 288), (4096, 4096), (544, 14336), (20000, 512)])
+def test_a_few_tokens_quantised_inside_the_product(m, n, k):
+    # the same bits as from the quantised activations, gated or not, with blocks of zeros, huge values and NaNs among them
+    from purlin_b200.ops.mx4 import mx4_gemm, mx4_gemm_swiglu, quantize_mx4
+    x = _rand(m, k, 30 + m, spread=8.0)
+    x[m - 1, :32] = 0
+    x[0, k - 1] = 3e38
+    w = quantize_mx4(_rand(n, k, 31))
+    q = quantize_mx4(x)
+    assert torch.equal(mx4_gemm(x, w), mx4_gemm(q, w))
+    if n % 32 == 0:
+        assert torch.equal(mx4_gemm_swiglu(x, w).nan_to_num(nan=7.0), mx4_gemm_swiglu(q, w).nan_to_num(nan=7.0))
+    x[m // 2, k // 2] = float("nan")
+    got, want = mx4_gemm(x, w), mx4_gemm(quantize_mx4(x), w)
+    assert got[m // 2].isnan().all() and torch.equal(got.nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))

@@ -98,3 +98,7 @@ def test_c_entries_refuse_without_a_launch():
     refused(lib.purlin_mx4_gemm(p, p, p, p, p, i(4), i(48), i(64), i(1), n, n))
     refused(lib.purlin_mx4_gemm(p, p, p, p, p, i(4), i(64), i(64), i(2), n, n))
     refused(lib.purlin_mx4_gemm(p, p, p, n, p, i(4), i(64), i(64), i(0), n, n))
+    refused(lib.purlin_mx4_linear(n, i(0), n, p, p, p, i(4), i(64), i(64), i(0), n, n))
+    refused(lib.purlin_mx4_linear(C.c_void_p(4098), i(0), n, p, p, p, i(4), i(64), i(64), i(0), n, n))
+    refused(lib.purlin_mx4_linear(p, i(0), n, p, p, p, i(400), i(64), i(64), i(0), n, n))      # no workspace
+    refused(lib.purlin_mx4_linear(p, i(0), n, p, p, p, i(4), i(60), i(64), i(0), n, n))
