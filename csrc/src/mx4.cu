@@ -36,8 +36,8 @@ constexpr int kScaleRows = 128, kScaleCols = 128, kScaleBytes = 512;
 // Four lanes have the 32 values of a block (8 each, 16 bytes of bf16 or fp16), a warp 256 columns, and a step of a warp is four of those side by
 // side in one row. The scale needs the exponent of the largest magnitude only, a byte, so the four blocks of a lane travel through the
 // shuffles in one word, and four more shuffles' worth of bytes become the words of the scales' layout in two. With one shuffle chain per block and
-// 64-bit index arithmetic the instructions, not the memory, were the bound. One B200, 8192 x 8192 bf16: 28.6 us, 5.9 TB/s (0.91 of a copy);
-// the way back 33 us, 5.1 TB/s; there and back with one chain per block 104 us.
+// 64-bit index arithmetic the instructions, not the memory, were the bound. One B200, 8192 x 8192 bf16: 27.3 us, 6.2 TB/s (0.95 of a copy);
+// the way back 24.8 us; 14336 x 8192 fp32 78.5 us, 6.8 TB/s; with one chain per block 8192 x 8192 took 104 us there and back.
 constexpr int kVec = 8, kWarpCols = 32 * kVec, kQuantThreads = 256, kUnroll = 4, kStepCols = kUnroll * kWarpCols;
 
 PURLIN_D uint4 ldOnce(const void* p) {
@@ -191,10 +191,11 @@ __global__ void __launch_bounds__(kQuantThreads) dequantizeKernel(const unsigned
       }
       if constexpr (TYPE == PURLIN_MX4_FP32) {
         float4* to = reinterpret_cast<float4*>(out + (at + size_t(u * kWarpCols)) * 4);
-        to[0] = make_float4(f[0], f[1], f[2], f[3]);
-        to[1] = make_float4(f[4], f[5], f[6], f[7]);
+        __stcs(to, make_float4(f[0], f[1], f[2], f[3]));
+        __stcs(to + 1, make_float4(f[4], f[5], f[6], f[7]));
       } else {
-        *reinterpret_cast<uint4*>(out + (at + size_t(u * kWarpCols)) * 2) = make_uint4(skinny::pack2(f[0], f[1]), skinny::pack2(f[2], f[3]), skinny::pack2(f[4], f[5]), skinny::pack2(f[6], f[7]));
+        __stcs(reinterpret_cast<uint4*>(out + (at + size_t(u * kWarpCols)) * 2),
+               make_uint4(skinny::pack2(f[0], f[1]), skinny::pack2(f[2], f[3]), skinny::pack2(f[4], f[5]), skinny::pack2(f[6], f[7])));
       }
     }
   }
@@ -253,7 +254,7 @@ template <int CTAS> PURLIN_D void commit(uint32_t elected, uint32_t bar) {      
     asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(elected) : "memory");
 }
 
-struct alignas(64) Maps { CUtensorMap a, b, sa, sb, c; };
+struct alignas(64) Maps { CUtensorMap a, b, sa, sb, c, bCut; };      // bCut: b in the boxes of a cut tile
 
 // Scales as [row blocks][rows of 128 bytes, four to a block of 512]: eight of those, of one or two row blocks
 PURLIN_D void loadScales(uint32_t smemDst, const CUtensorMap* map, int y, int rowBlock, uint32_t clusterBarAddress) {
@@ -277,9 +278,9 @@ constexpr size_t kWideSmem = size_t(kWideStages) * kWideStage + kWideStaging + k
 static_assert(kWideSmem <= size_t(kSmemLimit) && kWideStage % 1024 == 0, "the ring and the staging tiles fit one CTA per SM");
 
 struct WideParams {
-  int M, N, K, bn;                    // bn: columns of a tile, a multiple of 64 (of 128 where its last wave is halved), so they lie in two row blocks of W's scales
+  int M, N, K, bn;                    // bn: columns of a tile, a multiple of 64, so they lie in two row blocks of W's scales
   int tilesM, tilesN, items, fullItems;
-  int boxRows;                        // rows of W to a load: a CTA's half of a tile, or of half a tile where there are such
+  int cut;                            // items [fullItems, items) are the tiles of a small last wave, cut into so many parts (1, 2 or 4) of 64 columns or more
   uint32_t* status;
   uint64_t timeoutNs;
 };
@@ -287,11 +288,12 @@ struct WideParams {
 struct WideItem { int row0, col0, cols; };     // first row of the pair's 256, first column and number of columns
 constexpr int kBand = 8;
 PURLIN_D WideItem wideItem(const WideParams& p, int it) {
-  const int tile = it < p.fullItems ? it : p.fullItems + ((it - p.fullItems) >> 1);
+  const bool whole = it < p.fullItems;
+  const int tile = whole ? it : p.fullItems + (it - p.fullItems) / p.cut;
   const int perBand = kBand * p.tilesN, band = tile / perBand, within = tile - band * perBand, first = band * kBand;
   const int rows = min(p.tilesM - first, kBand);
   WideItem w{(first + within % rows) * 2 * kBM, within / rows * p.bn, p.bn};
-  if (it >= p.fullItems) { w.cols = p.bn / 2; w.col0 += ((it - p.fullItems) & 1) * w.cols; }
+  if (!whole) { w.cols = p.bn / p.cut; w.col0 += (it - p.fullItems) % p.cut * w.cols; }
   return w;
 }
 
@@ -349,8 +351,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4WideKernel(const __grid_co
         if (elected) {
           if (ctaRank == 0) tc::mbarExpectTx(fullBar(st), bytes);
           tc::tmaLoad2dPair(sA, &maps.a, kb * 128, aRow, full);
-          tc::tmaLoad2dPair(sB, &maps.b, kb * 128, bRow, full);
-          if (half > p.boxRows) tc::tmaLoad2dPair(sB + uint32_t(p.boxRows * 128), &maps.b, kb * 128, bRow + p.boxRows, full);
+          tc::tmaLoad2dPair(sB, it < p.fullItems ? &maps.b : &maps.bCut, kb * 128, bRow, full);
           loadScales(sS, &maps.sa, 8 * kb, sa, full);
           loadScales(sS + kScaleStage, &maps.sb, 8 * kb, sb, full);
         }
@@ -708,7 +709,7 @@ int launchRows(void (*kernel)(A...), uint32_t total, const Device& dev, cudaStre
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
   constexpr int kWarps = kQuantThreads / 32;
-  cfg.gridDim = dim3(std::min((total + kWarps - 1) / kWarps, uint32_t(dev.sms) * 8u));
+  cfg.gridDim = dim3(std::min((total + kWarps - 1) / kWarps, uint32_t(dev.sms) * 32u));      // (8 per SM, all resident at once: 5 to 20 % slower)
   cfg.blockDim = dim3(kQuantThreads); cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 1;
   return launched(cudaLaunchKernelEx(&cfg, kernel, args...)) ? 0 : 1;
 }
@@ -835,24 +836,26 @@ int launchWide(const void* aData, const void* aScales, const void* wData, const 
   WideParams p{};
   p.M = M; p.N = N; p.K = K; p.status = status; p.timeoutNs = 2ull * 1000 * 1000 * 1000;
   p.tilesM = (M + 2 * kBM - 1) / (2 * kBM);
-  // the width that is expected to take least: a tile costs its columns and about 48 columns' worth besides (fill, drain, the loads of A)
+  // The width that is expected to take least: a tile costs its columns and about 48 columns' worth besides (fill, drain, the loads of A). Tiles of a
+  // last wave that leaves pairs idle are cut where every part finds a pair (us, uncut / in halves / in quarters:
+  // 1000 x 14336 x 8192 gated 50.9 / 46.0 / 45.7, 4096 x 4864 x 2048 20.7 / 19.3 / 19.0).
   double least = 1e30;
   for (int bn : {256, 192, 128}) {
     const int tilesN = (N + bn - 1) / bn, tiles = p.tilesM * tilesN, rest = tiles % pairs;
-    const bool halved = bn % 128 == 0 && tiles > pairs && rest > 0 && 2 * rest <= pairs;
-    const double cost = double(tiles / pairs) * (bn + 48) + (rest ? (halved ? bn / 2 : bn) + 48 : 0);
+    const int cut = tiles <= pairs || !rest ? 1 : bn == 256 && 4 * rest <= pairs ? 4 : bn != 192 && 2 * rest <= pairs ? 2 : 1;
+    const double cost = double(tiles / pairs) * (bn + 48) + (rest ? bn / cut + 48 : 0);
     if (cost < least) {
       least = cost;
-      p.bn = bn; p.tilesN = tilesN;
-      p.fullItems = halved ? tiles - rest : tiles;
-      p.items = halved ? p.fullItems + 2 * rest : tiles;
-      p.boxRows = halved ? bn / 4 : bn / 2;
+      p.bn = bn; p.tilesN = tilesN; p.cut = cut;
+      p.fullItems = cut > 1 ? tiles - rest : tiles;
+      p.items = p.fullItems + (tiles - p.fullItems) * cut;
     }
   }
   const int outCols = swiglu ? N / 2 : N;
   Maps maps{};
   if (!makeTensorMap(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, aData, uint64_t(M), uint64_t(K) / 2, uint64_t(K) / 2, kBM) ||
-      !makeTensorMap(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, wData, uint64_t(N), uint64_t(K) / 2, uint64_t(K) / 2, uint32_t(p.boxRows)) ||
+      !makeTensorMap(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, wData, uint64_t(N), uint64_t(K) / 2, uint64_t(K) / 2, uint32_t(p.bn / 2)) ||
+      !(p.cut == 1 || makeTensorMap(&maps.bCut, CU_TENSOR_MAP_DATA_TYPE_UINT8, wData, uint64_t(N), uint64_t(K) / 2, uint64_t(K) / 2, uint32_t(p.bn / 2 / p.cut))) ||
       !scaleMap(&maps.sa, aScales, M, K, 1) || !scaleMap(&maps.sb, wScales, N, K, 2) ||
       !outputMap(&maps.c, C, uint64_t(M), uint64_t(outCols))) return 1;
   cfg.gridDim = dim3(unsigned(2 * std::min(pairs, p.items))); cfg.numAttrs = 2;
