@@ -53,7 +53,9 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
     const Tensor &x = s[0], &wGateUp = s[1], &wDown = s[2], &h = s[3], &saved = s[4];
-    const int64_t needs = ctx->saved_data["needs"].toInt(), tokens = x.size(0), hidden = wDown.size(0), intermediate = wDown.size(1);
+    int64_t needs = ctx->saved_data["needs"].toInt();
+    for (int i = 0; i < 3; ++i) if (!ctx->needs_input_grad(size_t(i))) needs &= ~(int64_t(1) << i);      // (a pass that asks for some of them only)
+    const int64_t tokens = x.size(0), hidden = wDown.size(0), intermediate = wDown.size(1);
     Tensor dx, dGateUp, dDown, dz;
     if (!grads[0].defined()) return {dx, dGateUp, dDown, Tensor()};
     const bool again = at::GradMode::is_enabled() && (grads[0].requires_grad() || needs);

@@ -189,7 +189,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
     import sysconfig
 
     import torch
-    build_cuda(force, verbose)
+    build_cuda(verbose=verbose)
     home = Path(torch.__file__).resolve().parent
     src = CSRC / "src" / "torch_ops.cpp"
     cuda_include = str(Path(_nvcc()).resolve().parent.parent / "include")

@@ -49,3 +49,24 @@ class Mx4MLP:
 
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         return mx4_gemm(mx4_gemm_swiglu(x, self.w_gu), self.w_down, out)
+
+
+def smoke_gated_mlp():
+    """A tiny training step on one GPU against fp32 autograd, then the block in 4 bits."""
+    from ..ops.gated_ffn import split_gate_up
+    mlp = GatedMLP(hidden=512, intermediate=1024, device="cuda:0")
+    g = torch.Generator(device="cuda:0").manual_seed(3)
+    x = torch.randn(200, 512, generator=g, device="cuda:0").to(torch.bfloat16)
+    y = mlp(x)
+    y.backward(torch.ones_like(y))
+    gate, up = (w.detach().float().requires_grad_() for w in split_gate_up(mlp.w_gu))
+    down = mlp.w_down.detach().float().requires_grad_()
+    ref = (torch.nn.functional.silu(x.float() @ gate.t()) * (x.float() @ up.t())) @ down.t()
+    ref.backward(torch.ones_like(ref))
+    d_gate, d_up = split_gate_up(mlp.w_gu.grad)
+    served = mlp.quantized()(x)
+    torch.cuda.synchronize()
+    for got, want in ((y, ref), (d_gate, gate.grad), (d_up, up.grad), (mlp.w_down.grad, down.grad)):
+        err = ((got.float() - want).norm() / want.norm()).item()
+        assert err < 1e-2, f"gated MLP smoke mismatch: {err}"
+    assert torch.isfinite(served).all()

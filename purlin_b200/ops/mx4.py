@@ -26,7 +26,7 @@ class Mx4Tensor:
     """A [rows, cols] tensor in 4-bit microscaled form. ``data``: uint8 [rows, cols / 2], the even column in a byte's low half. ``scales``: uint8, a
     byte b per 32 columns of a row for 2^(b - 127) (255: the block stands for NaNs), in the tensor cores' order: blocks of 512 bytes for
     128 rows x 128 columns, [rows / 128][cols / 128][row % 32][row / 32 % 4][col / 32 % 4], zeros past the edges."""
-    __slots__ = ("data", "scales")
+    __slots__ = ("data", "scales", "shape", "device")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor):
         if data.dtype != torch.uint8 or scales.dtype != torch.uint8:
@@ -39,21 +39,13 @@ class Mx4Tensor:
             raise ValueError("data and scales must start on a 16-byte boundary")
         if data.shape[0] > MAX_ROWS:
             raise ValueError("at most 2^30 rows")
-        self.data, self.scales = data, scales
+        self.data, self.scales, self.shape, self.device = data, scales, (data.shape[0], 2 * data.shape[1]), data.device
 
     @classmethod
-    def _of(cls, data: torch.Tensor, scales: torch.Tensor) -> "Mx4Tensor":
+    def _of(cls, data: torch.Tensor, scales: torch.Tensor, rows: int, cols: int) -> "Mx4Tensor":
         q = cls.__new__(cls)                 # (what the quantisation made needs no check)
-        q.data, q.scales = data, scales
+        q.data, q.scales, q.shape, q.device = data, scales, (rows, cols), data.device
         return q
-
-    @property
-    def shape(self) -> Tuple[int, int]:
-        return self.data.shape[0], 2 * self.data.shape[1]
-
-    @property
-    def device(self) -> torch.device:
-        return self.data.device
 
     def scale_matrix(self) -> torch.Tensor:
         """The scales' bytes in the order of the values, uint8 [rows, cols / 32]."""
@@ -68,50 +60,54 @@ class Mx4Tensor:
         return _native.torch_ops().mx4_dequantize(self.data, self.scales, TYPES[dtype])
 
 
-def _check_dense(x: torch.Tensor):
-    if x.dtype not in TYPES:
+def _check_dense(x: torch.Tensor) -> Tuple[int, int, int]:
+    """Rows, columns and type number of a dense operand."""
+    kind = TYPES.get(x.dtype)
+    if kind is None:
         raise TypeError("quantisation takes bf16, fp16 or fp32 values")
-    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
+    shape = x.shape
+    cols = shape[-1] if shape else 0
+    if cols == 0 or cols % 32:
         raise ValueError("the last dimension must be a multiple of 32")
     if not (x.is_cuda and x.is_contiguous()):
         raise ValueError("operands must be contiguous CUDA tensors")
     if x.data_ptr() % 16:
         raise ValueError("operands must start on a 16-byte boundary")
-    if x.numel() // x.shape[-1] > MAX_ROWS:
+    rows = x.numel() // cols
+    if rows > MAX_ROWS:
         raise ValueError("at most 2^30 rows")
+    return rows, cols, kind
 
 
 def quantize_mx4(x: torch.Tensor) -> Mx4Tensor:
     """``x [..., cols]`` (bf16, fp16 or fp32, contiguous, cols a multiple of 32) as an ``Mx4Tensor`` of its rows. A block's power of two is that of its
     largest magnitude over 4, at least 2^-127; values are rounded to the nearest of the format, ties to the even code, and above 6 times the power
     to 6. A block that holds an infinity or a NaN stands for NaNs."""
-    _check_dense(x)
-    cols = x.shape[-1]
-    return Mx4Tensor._of(*_native.torch_ops().mx4_quantize(x, TYPES[x.dtype], x.numel() // cols, cols))
+    rows, cols, kind = _check_dense(x)
+    return Mx4Tensor._of(*_native.torch_ops().mx4_quantize(x, kind, rows, cols), rows, cols)
 
 
 def _product(a: Union[torch.Tensor, Mx4Tensor], w: Mx4Tensor, out: Optional[torch.Tensor], epilogue: int) -> torch.Tensor:
     if not isinstance(w, Mx4Tensor):
         raise TypeError("w is an Mx4Tensor (quantize_mx4)")
-    quantised = isinstance(a, Mx4Tensor)
-    if not quantised:
-        _check_dense(a)
     n, k = w.shape
-    device = w.data.device
-    shape = a.shape
-    if shape[-1] != k or a.device != device:
+    if isinstance(a, Mx4Tensor):
+        rows, cols = a.shape
+        operand = (a.data, 0, a.scales)
+    else:
+        rows, cols, kind = _check_dense(a)
+        operand = (a, kind, None)
+    if cols != k or a.device != w.device:
         raise ValueError("a is [..., K] and w is [N, K], on one device")
     if n == 0 or n % (32 if epilogue == EPI_SWIGLU else 8):
         raise ValueError("the SwiGLU epilogue needs N to be a multiple of 32 (16 rows of gate and 16 of up in turn)" if epilogue == EPI_SWIGLU
                          else "N must be a multiple of 8")
-    rows = shape[0] if quantised else a.numel() // k
-    shape = (*shape[:-1], n // 2 if epilogue == EPI_SWIGLU else n)
-    operand = (a.data, 0, a.scales) if quantised else (a, TYPES[a.dtype], None)
+    shape = (*a.shape[:-1], n // 2 if epilogue == EPI_SWIGLU else n)
     if out is None:
         return _native.torch_ops().mx4_new_product(*operand, w.data, w.scales, shape, rows, epilogue)
     if out.dtype != torch.bfloat16:
         raise TypeError("out is a bf16 tensor")
-    if out.shape != shape or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
+    if out.shape != shape or out.device != w.device or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"out is a contiguous tensor of {shape} on the operands' device")
     if rows:
         _native.torch_ops().mx4_product(*operand, w.data, w.scales, out, rows, epilogue)

@@ -146,6 +146,55 @@ def test_only_the_gradients_that_are_asked_for(t, h, i, mask):
             assert leaf.grad is None
 
 
+def test_some_of_the_gradients_and_a_second_pass_over_a_kept_graph():
+    from purlin_b200.ops.gated_ffn import gated_ffn
+    args = _inputs(300, 264, 528, seed=14)
+    want, off = _oracle(*args, "silu")
+    leaves = [v.clone().requires_grad_() for v in args[:3]]
+    y = gated_ffn(*leaves)
+    first = torch.autograd.grad(y, leaves, args[3], retain_graph=True)
+    for n in range(3):
+        (one,) = torch.autograd.grad(y, leaves[n], args[3], retain_graph=True)
+        assert ((one.double() - want[n + 1]).abs() <= off[n + 1]).all()
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, args[3]), first))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, leaves, args[3])
+
+
+def test_under_checkpointing_and_from_threads():
+    # the forward runs again in the backward's thread; two host threads call at once, each on a stream of its own
+    import threading
+
+    from torch.utils.checkpoint import checkpoint
+
+    from purlin_b200.ops.gated_ffn import gated_ffn
+    args = _inputs(300, 264, 528, seed=15)
+    want = _run(*args, "silu")
+    for reentrant in (False, True):
+        leaves = [v.clone().requires_grad_() for v in args[:3]]
+        y = checkpoint(gated_ffn, *leaves, use_reentrant=reentrant)
+        y.backward(args[3])
+        assert all(torch.equal(p.grad, q) for p, q in zip(leaves, want[1:]))
+    others = [_inputs(100 + 50 * n, 264, 272, seed=16 + n) for n in range(2)]
+    wants = [_run(*a, "gelu") for a in others]
+    torch.cuda.synchronize()
+    right = [0, 0]
+
+    def work(n):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = _run(*others[n], "gelu")
+                torch.cuda.current_stream().synchronize()
+                right[n] += all(torch.equal(p, q) for p, q in zip(got, wants[n]))
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert right == [20, 20]
+
+
 def test_without_gradients_nothing_is_kept_and_the_values_are_the_same_operator():
     from purlin_b200.ops.gated_ffn import gated_ffn
     for activation in ("silu", "gelu"):
