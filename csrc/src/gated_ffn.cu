@@ -25,6 +25,7 @@
 #include <string>
 #include <type_traits>
 
+#include "purlin/ffn_schedule.hpp"
 #include "purlin/gated_ffn.h"
 #include "purlin/gemm.h"
 #include "purlin/gemm_skinny.cuh"
@@ -33,10 +34,10 @@
 #include "purlin/tensor_map.hpp"
 
 using namespace purlin;
+using namespace purlin::ffn;
 
 namespace {
 
-constexpr int kBM = 128, kBK = 64;
 constexpr int kBoxBytes = 64 * 128;             // a box of 64 x 64 of an operand whose rows or columns are contiguous
 constexpr int kAccStride = 256, kTmemCols = 512;
 constexpr int kEpiWarps = 8, kThreads = 32 * (2 + kEpiWarps);
@@ -49,25 +50,17 @@ constexpr int kSavedVectors = 6;                // 16-byte pieces of 32 values i
 constexpr size_t kSavedBlock = size_t(kSavedVectors) * 32 * 16;   // 32 rows x 32 columns
 static_assert(8 * (2 * kMaxStages + 4) + 8 <= kBarrierBytes, "the barriers, the TMEM base and the abort word fit their block");
 
-enum { kStore = 0, kGate = 1, kGateGrad = 2 };
-
 // One product. A launch has one, or the three gradients, which need one another as little as their tiles do.
 struct alignas(64) Group {
   CUtensorMap a, b, c;
-  int M, N, K, tilesM, tilesN;
+  Tiles t;                               // (with t.split above 1 the sums go to `partial` and finishKernel adds them up)
   int aMn;                               // m is contiguous in A (k otherwise)
   int aBytes;                            // that one block of A brings into a stage: fewer than 128 rows of it where there are fewer
-  int split;                             // parts of k, a tile of work each; above 1 the sums go to `partial` and finishKernel adds them up
 };
-// Work [start, start + count) of a group (tiles, times the parts of k; with `halves` their accumulators one by one, 2 * count of them) in turn over
-// `pairs` CTA pairs (or CTAs) from number `first` on, wrapping around.
-struct Segment { int group, start, count, first, pairs, halves; };
-constexpr int kMaxGroups = 3, kMaxSegments = 3 * kMaxGroups;
 
 struct alignas(64) Params {
   Group g[kMaxGroups];
-  Segment seg[kMaxSegments];
-  int segments;
+  Schedule schedule;
   int bn, stages, aBytes;                // aBytes: room of one block of A in a stage
   uint4* saved;                          // pre-activations: written by kGate (unless null), read by kGateGrad
   int savedCols;                         // its 32-column blocks per row block
@@ -171,50 +164,7 @@ template <int CTAS> PURLIN_D void commit(uint32_t elected, uint32_t bar) {      
     asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(elected) : "memory");
 }
 
-// Tile t -> (row block, column block), rows fastest inside bands of row blocks: the tiles in flight share operands in L2
-constexpr int kBand = 8;
-PURLIN_D void tileCoord(const Group& g, int t, int& mIdx, int& nIdx) {
-  const int perBand = kBand * g.tilesN, band = t / perBand, within = t - band * perBand, first = band * kBand;
-  const int rows = min(g.tilesM - first, kBand);
-  mIdx = first + within % rows;
-  nIdx = within / rows;
-}
-// first row of the pair's accumulators, first column, number of accumulators
-struct Item { int group, tile, part, row, col, count; };
 constexpr int kPartialBlock = 8 * 32;    // 32 rows x 32 columns of partial sums in 16-byte pieces: eight for every lane (a row), 512 bytes side by side
-struct KRange { int begin, end; };       // k-blocks of a part
-PURLIN_D KRange kRangeOf(const Group& g, int part) {
-  const int blocks = (g.K + kBK - 1) / kBK;
-  return KRange{int(int64_t(blocks) * part / g.split), int(int64_t(blocks) * (part + 1) / g.split)};
-}
-// The work of pair `idx` of `units`, in the order in which all warps walk it; body returns false to stop.
-template <int CTAS, int ACCS, typename F> PURLIN_D void forItems(const Params& p, int idx, int units, F&& body) {
-  for (int s = 0; s < p.segments; ++s) {
-    const Segment& seg = p.seg[s];
-    const Group& g = p.g[seg.group];
-    const int at = idx - seg.first + (idx < seg.first ? units : 0);
-    if (at >= seg.pairs) continue;
-    const int n = ACCS == 2 && seg.halves ? 2 * seg.count : seg.count;
-    for (int i = at; i < n; i += seg.pairs) {
-      Item m;
-      int mIdx, nIdx, first = 0;
-      m.group = seg.group;
-      m.tile = seg.start + (ACCS == 2 && seg.halves ? i >> 1 : i);
-      m.part = 0;
-      if (g.split > 1) { const int tiles = g.tilesM * g.tilesN; m.part = m.tile / tiles; m.tile -= m.part * tiles; }
-      tileCoord(g, m.tile, mIdx, nIdx);
-      m.count = 1;
-      if constexpr (ACCS == 2) {
-        if (seg.halves) first = i & 1;
-        else m.count = (mIdx * ACCS + 1) * CTAS * kBM < g.M ? 2 : 1;      // rows of the last tile that end in its first accumulator
-      }
-      m.row = (mIdx * ACCS + first) * CTAS * kBM;
-      m.col = nIdx * p.bn;
-      if (m.row < g.M && !body(m)) return;
-    }
-  }
-}
-
 // CTAS = 2: a cluster of two CTAs owns a tile: each loads its 128 rows of A per accumulator and its half of B's columns, CTA 0 issues one
 // 256-row MMA for the pair. ACCS = 2: a tile is two accumulators tall; they share B, and their MMAs alternate (an MMA waits for the one before
 // into the same columns). ACCS = 1: tiles alternate between the two accumulators, the epilogue of one runs under the MMAs of the next.
@@ -260,16 +210,17 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
   tc::gridLaunchDependents();
   const uint32_t tmemBase = *tmemBaseWord;
   const uint32_t leaderBars = CTAS == 2 ? tc::mapToCta(barBase, 0) : barBase;
+  auto groupOf = [&](int i) -> const Tiles& { return p.g[i].t; };
   constexpr bool kAnyA = EPI == kStore;       // A's order goes by the product (k is contiguous in the others)
 
   if (warp == 0) {
     // ---- TMA producer ----
     const uint32_t elected = electOne();
     uint32_t st = 0, ph = 0;
-    forItems<CTAS, ACCS>(p, pairIdx, numPairs, [&](const Item& m) {
+    forItems<CTAS, ACCS>(p.schedule, p.bn, pairIdx, numPairs, groupOf, [&](const Item& m) {
       const Group& g = p.g[m.group];
       const int aRow = m.row + int(ctaRank) * kBM, bRow = m.col + int(ctaRank) * bnLocal;
-      const KRange k = kRangeOf(g, m.part);
+      const KRange k = kRangeOf(g.t, m.part);
       const bool aMn = kAnyA && g.aMn;
       const uint32_t bytes = uint32_t(CTAS * (m.count * g.aBytes + bBytes));
       for (int kb = k.begin; kb < k.end; ++kb) {
@@ -316,9 +267,9 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
       constexpr uint32_t kStepB = B_MN ? kStepMn : kStepK;
       const uint32_t stageStep = stageBytes >> 4, accStep = uint32_t(p.aBytes) >> 4;
       uint32_t st = 0, ph = 0, accIt = 0, use0 = 0, use1 = 0;
-      forItems<CTAS, ACCS>(p, pairIdx, numPairs, [&](const Item& m) {
+      forItems<CTAS, ACCS>(p.schedule, p.bn, pairIdx, numPairs, groupOf, [&](const Item& m) {
         const Group& g = p.g[m.group];
-        const KRange range = kRangeOf(g, m.part);
+        const KRange range = kRangeOf(g.t, m.part);
         const int a0 = ACCS == 1 ? int(accIt & 1) : 0;
         const bool two = ACCS == 2 && m.count == 2;
         bool ok = waitAll(tmemEmptyBar(a0), ((a0 ? use1 : use0) & 1) ^ 1, abortWord, p.timeoutNs);
@@ -365,17 +316,17 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
     const uint32_t stagingWarp = stagingAll + uint32_t(warp - 2) * uint32_t(kStageTiles * kStageTileBytes);
     const uint32_t rowAddr = uint32_t(lane) * 128u, swz = uint32_t(lane & 7);
     uint32_t accIt = 0, uses = 0, tileCount = 0;
-    forItems<CTAS, ACCS>(p, pairIdx, numPairs, [&](const Item& m) {
+    forItems<CTAS, ACCS>(p.schedule, p.bn, pairIdx, numPairs, groupOf, [&](const Item& m) {
       const uint32_t number = accIt++;
       if (ACCS == 1 ? int(number & 1) != group : group >= m.count) return true;
       const Group& g = p.g[m.group];
       const int row0 = m.row + ((ACCS == 2 ? group : 0) * CTAS + int(ctaRank)) * kBM + quarter * 32;
-      const int n0 = m.col, rowsValid = min(g.M - row0, 32);
+      const int n0 = m.col, rowsValid = min(g.t.M - row0, 32);
       // chunks of 32 accumulator columns that hold output
-      const int nChunks = rowsValid <= 0 ? 0 : (min(p.bn, g.N - n0) + 31) / 32;
+      const int nChunks = rowsValid <= 0 ? 0 : (min(p.bn, g.t.N - n0) + 31) / 32;
       uint4* saved = nullptr;                                           // of this warp's rows and the tile's first columns
       uint32_t z[24], z1[24] = {};
-      const int blocks = min(p.bn, g.N - n0) / 16;                      // kGateGrad: saved blocks of this tile (N is a multiple of 16)
+      const int blocks = min(p.bn, g.t.N - n0) / 16;                      // kGateGrad: saved blocks of this tile (N is a multiple of 16)
       if constexpr (EPI == kGate) { if (p.saved) saved = p.saved + (size_t(row0 / 32) * size_t(p.savedCols) + size_t(n0 / 32)) * (kSavedBlock / 16); }
       if constexpr (EPI == kGateGrad) {
         saved = p.saved + (size_t(row0 / 32) * size_t(p.savedCols) + size_t(n0 / 16)) * (kSavedBlock / 16);
@@ -402,8 +353,8 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
         __syncwarp();
         if (lane == 0) { tc::tmaStore2d(&g.c, col, row0, buf); tc::bulkCommitGroup(); }
       };
-      if (EPI == kStore && g.split > 1) {
-        const size_t block = ((size_t(m.part) * size_t(g.tilesM * g.tilesN) + size_t(m.tile)) * (ACCS * CTAS) + size_t((m.row / (CTAS * kBM) % ACCS + (ACCS == 2 && m.count == 2 ? group : 0)) * CTAS + int(ctaRank))) * 4 + size_t(quarter);
+      if (EPI == kStore && g.t.split > 1) {
+        const size_t block = ((size_t(m.part) * size_t(g.t.tilesM * g.t.tilesN) + size_t(m.tile)) * (ACCS * CTAS) + size_t((m.row / (CTAS * kBM) % ACCS + (ACCS == 2 && m.count == 2 ? group : 0)) * CTAS + int(ctaRank))) * 4 + size_t(quarter);
         float4* to = p.partial + block * size_t(p.bn / 32) * kPartialBlock + lane;
 #pragma unroll 1
         for (int c = 0; c < nChunks; ++c) {
@@ -512,7 +463,7 @@ __global__ void __launch_bounds__(kFinishThreads) finishKernel(const float4* __r
   const int chunks = bn / 32, c = int(w % chunks);
   const int64_t block = w / chunks;                            // tile, then accumulator, CTA and quarter: blocksM blocks of 32 rows
   const int tile = int(block / blocksM), rowBlock = int(block % blocksM);
-  Group g;
+  Tiles g{};
   g.tilesM = tilesM; g.tilesN = tilesN;
   int mIdx, nIdx;
   tileCoord(g, tile, mIdx, nIdx);
@@ -544,8 +495,6 @@ __global__ void __launch_bounds__(kFinishThreads) finishKernel(const float4* __r
 // ------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------
-struct Shape { int ctas, accs, bn, split; };     // split: parts of the first product's k
-
 struct Device { int sms = 0, index = -1; };
 bool currentDevice(Device& d) {
   static std::mutex mu;
@@ -555,102 +504,6 @@ bool currentDevice(Device& d) {
   if (!sms[d.index]) cudaDeviceGetAttribute(&sms[d.index], cudaDevAttrMultiProcessorCount, d.index);
   d.sms = sms[d.index];
   return d.sms > 0;
-}
-
-struct Sizes { int M, N, K; };
-int64_t tilesOf(const Sizes& z, const Shape& s) {
-  const int tileRows = kBM * s.ctas * s.accs;
-  return int64_t((z.M + tileRows - 1) / tileRows) * ((z.N + s.bn - 1) / s.bn);
-}
-// Expected cycles of a tile. A k-block (64 of k) takes the longer of its MMAs (bn / 2 cycles per 16 of k and accumulator, a little more where they
-// all go into one) and its loads from L2 (about 56 bytes a cycle and SM). The epilogue follows the main loop of a tile of two accumulators and
-// hides under the next one's with one. us under the power cap, 512 x 256 / 256 x 256 per pair / 128 x 256 per CTA: gradient of the gate 1000 x 3584,
-// k 8192 99 / 66 / 79; 8192 x 4096, k 1024 124 / 113 / 110; gate and up 4099 x 4096, k 7168 201 / 216 / 262; 2595 x 46560, k 424 196 / 183 / 219.
-double tileCycles(const Sizes& z, const Shape& s, int epi) {
-  const double kBlocks = (z.K + kBK - 1) / kBK;
-  const double mma = 4.0 * s.accs * s.bn / 2 * (s.accs == 2 ? 1.0 : 1.08);
-  const double load = (s.accs * std::min(z.M, kBM) + s.bn / s.ctas) * 128.0 / 56;
-  const double column = epi == kStore ? (s.accs == 2 ? 16 : 10) : epi == kGate ? (s.accs == 2 ? 46 : s.ctas == 2 ? 40 : 50) : s.accs == 2 ? 140 : s.ctas == 2 ? 75 : 80;
-  const double epilogue = s.bn * column, main = kBlocks * std::max(mma, load);
-  return s.accs == 2 ? main + 1500 + epilogue : std::max(main + 500, epilogue + 1200);
-}
-size_t partialBytes(const Sizes& z, const Shape& s) { return s.split > 1 ? size_t(s.split) * size_t(tilesOf(z, s)) * size_t(kBM * s.ctas * s.accs) * size_t(s.bn) * 4 : 0; }
-constexpr int kMaxSplit = 16;
-constexpr size_t kMaxPartial = size_t(256) << 20;
-// The tile that is expected to take least, and the parts into which k of the first product is cut (where `mayCut`): its tiles may be few and long.
-// The gradient of x, [tokens, hidden], sums over twice the intermediate size: 2595 x 424 with k = 46560 has 12 tiles (all three gradients, us, whole /
-// cut: 2595, 424, 23280 375 / 281; 16, 8192, 28672 530 / 511; 100, 1024, 2048 22.0 / 16.9).
-Shape chooseShape(const Sizes* z, int n, int sms, int epi, bool mayCut) {
-  Shape best{2, 2, 256, 1};
-  double least = 1e30;
-  auto consider = [&](Shape s) {
-    const int units = sms / s.ctas;
-    for (s.split = 1; s.split <= (mayCut ? kMaxSplit : 1); s.split *= 2) {
-      const Sizes first{z[0].M, z[0].N, (z[0].K + s.split - 1) / s.split};
-      if (s.split > 1 && (first.K < 4 * kBK || partialBytes(z[0], s) > kMaxPartial)) break;
-      double cycles = 0, longest = 0;
-      if (n == 1) {
-        const int64_t tiles = tilesOf(z[0], s) * s.split, rest = tiles % units;
-        double waves = double((tiles + units - 1) / units);
-        if (s.accs == 2 && tiles > units && rest > 0 && 2 * rest <= units) waves -= 0.5;
-        cycles = waves * tileCycles(first, s, epi);
-      } else {
-        double last = 0;
-        for (int i = 0; i < n; ++i) {
-          last = tileCycles(i ? z[i] : first, s, epi);
-          longest = std::max(longest, last);
-          cycles += double(tilesOf(z[i], s)) * (i ? 1 : s.split) * last / units;
-        }
-        cycles = std::max(cycles + 0.5 * last, longest);
-      }
-      if (s.accs == 1) cycles += 1500 + s.bn * 8.0;
-      if (s.split > 1) cycles += 4000 + double(partialBytes(z[0], s)) / 3000;     // a launch, and the parts written and read
-      if (cycles < least) { least = cycles; best = s; }
-    }
-  };
-  consider({2, 2, 256, 1});
-  consider({2, 2, 128, 1});
-  consider({2, 1, 256, 1});
-  consider({1, 1, 256, 1});
-  consider({1, 1, 128, 1});
-  if (epi != kGate) consider({1, 1, 64, 1});     // (64 columns of Z are 32 of h: half a staging tile)
-  return best;
-}
-
-// Shares the tiles of a launch out over its pairs: group by group, the longest tiles first; pairs that got one tile fewer than others take more
-// of the next group's. The last wave of all, if it fills at most half of the pairs, goes out as single accumulators.
-void shareOut(Params& p, int groups, const Shape& s, int units, int epi) {
-  int order[kMaxGroups] = {0, 1, 2};
-  double cost[kMaxGroups] = {};
-  for (int i = 0; i < groups; ++i) cost[i] = tileCycles(Sizes{p.g[i].M, p.g[i].N, (p.g[i].K + p.g[i].split - 1) / p.g[i].split}, s, epi);
-  std::sort(order, order + groups, [&](int a, int b) { return cost[a] > cost[b]; });
-  int lateFirst = 0, late = 0;                // pairs [lateFirst, lateFirst + late), wrapping around, end `ahead` cycles after the others
-  double ahead = 0;
-  auto add = [&](int group, int start, int count, int first, int pairs, int halves) {
-    if (count > 0) p.seg[p.segments++] = Segment{group, start, count, first % units, pairs, halves};
-  };
-  p.segments = 0;
-  for (int i = 0; i < groups; ++i) {
-    const int group = order[i], tiles = p.g[group].tilesM * p.g[group].tilesN * p.g[group].split;
-    int done = 0;
-    if (late > 0) {
-      const int each = int(ahead / cost[group] + 0.5);
-      done = int(std::min<int64_t>(tiles, int64_t(each) * (units - late)));
-      add(group, 0, done, lateFirst + late, units - late, 0);
-    }
-    const int left = tiles - done, whole = left / units * units, rest = left - whole;
-    add(group, done, whole, lateFirst + late, units, 0);
-    if (rest) {
-      const bool halves = i == groups - 1 && s.accs == 2 && 2 * rest <= units && (whole || done || i > 0);
-      add(group, done + whole, rest, lateFirst + late, halves ? 2 * rest : rest, halves);
-      lateFirst = (lateFirst + late) % units; late = rest; ahead = cost[group];
-    } else if (done && done % (units - late)) {
-      const int some = done % (units - late);
-      lateFirst = (lateFirst + late) % units; late = some; ahead = cost[group];
-    } else if (left > 0 || done) {
-      late = 0;
-    }
-  }
 }
 
 template <bool B_MN, int EPI, int CTAS, int ACCS>
@@ -679,14 +532,16 @@ int launchAs(Params& p, int groups, const Shape& s, const Device& dev, cudaStrea
   }
   int64_t tiles = 0;
   for (int i = 0; i < groups; ++i) {
-    const Sizes z{p.g[i].M, p.g[i].N, p.g[i].K};
+    const Sizes z{p.g[i].t.M, p.g[i].t.N, p.g[i].t.K};
     const int tileRows = kBM * CTAS * ACCS;
-    p.g[i].tilesM = (z.M + tileRows - 1) / tileRows; p.g[i].tilesN = (z.N + s.bn - 1) / s.bn;
-    if (tilesOf(z, s) * p.g[i].split > INT32_MAX / 4) { setError("feed-forward: the product is too large"); return 1; }
-    tiles += tilesOf(z, s) * p.g[i].split;
+    p.g[i].t.tilesM = (z.M + tileRows - 1) / tileRows; p.g[i].t.tilesN = (z.N + s.bn - 1) / s.bn;
+    if (tilesOf(z, s) * p.g[i].t.split > INT32_MAX / 4) { setError("feed-forward: the product is too large"); return 1; }
+    tiles += tilesOf(z, s) * p.g[i].t.split;
   }
   units = int(std::min<int64_t>(units, tiles));
-  shareOut(p, groups, s, units, EPI);
+  Tiles work[kMaxGroups];
+  for (int i = 0; i < groups; ++i) work[i] = p.g[i].t;
+  shareOut(p.schedule, work, groups, s, units, EPI);
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = CTAS; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -738,7 +593,7 @@ int run(const Product* products, int n, void* saved, void* partial, int activati
   for (int i = 0; i < n; ++i) {
     const Product& q = products[i];
     Group& g = p.g[i];
-    g.M = q.M; g.N = q.N; g.K = q.K; g.aMn = q.aMn; g.split = i ? 1 : s.split;
+    g.t.M = q.M; g.t.N = q.N; g.t.K = q.K; g.aMn = q.aMn; g.t.split = i ? 1 : s.split;
     // Few rows of A take only their own room in a stage: the MMA's other rows read what lies behind, and rows of the accumulator that are no
     // rows of the result are never stored.
     const int boxRows = q.aMn || s.ctas == 2 ? kBM : std::min(kBM, (q.M + 7) / 8 * 8);
@@ -754,13 +609,13 @@ int run(const Product* products, int n, void* saved, void* partial, int activati
                : s.ctas == 2 ? launchAs<B_MN, EPI, 2, 1>(p, n, s, dev, stream) : launchAs<B_MN, EPI, 1, 1>(p, n, s, dev, stream);
   if (rc || s.split == 1) return rc;
   const Group& g = p.g[0];
-  const int blocksM = s.ctas * s.accs * 4, tiles = g.tilesM * g.tilesN;
+  const int blocksM = s.ctas * s.accs * 4, tiles = g.t.tilesM * g.t.tilesN;
   const int64_t warps = int64_t(tiles) * blocksM * (s.bn / 32);
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(unsigned((warps + kFinishThreads / 32 - 1) / (kFinishThreads / 32))); cfg.blockDim = dim3(kFinishThreads); cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, finishKernel, static_cast<const float4*>(p.partial), static_cast<__nv_bfloat16*>(products[0].C), g.M, g.N, g.split, tiles, g.tilesM, g.tilesN,
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, finishKernel, static_cast<const float4*>(p.partial), static_cast<__nv_bfloat16*>(products[0].C), g.t.M, g.t.N, g.t.split, tiles, g.t.tilesM, g.t.tilesN,
                                            blocksM, s.bn, warps);
   if (e != cudaSuccess) { setError(std::string("feed-forward launch: ") + cudaGetErrorString(e)); return 1; }
   return 0;
