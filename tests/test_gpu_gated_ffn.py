@@ -380,3 +380,16 @@ def test_example():
     example = pathlib.Path(__file__).resolve().parent.parent / "examples" / "gated_mlp.py"
     done = subprocess.run([sys.executable, str(example), "200", "512", "1024"], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and done.stdout.strip().endswith("ok"), done.stdout + done.stderr      # it checks its own gradients
+
+
+def test_offsets_past_32_bits():
+    # 6.9 GB of saved pre-activations, 4.6 GB of dZ: the last tokens against the formula on them alone
+    from purlin_b200.ops.gated_ffn import gated_ffn
+    t, h, i = 20000, 64, 57344
+    x, w_gu, w_down, dy = _inputs(t, h, i, seed=20)
+    x.requires_grad_()
+    y = gated_ffn(x, w_gu, w_down)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    for rows in (slice(0, 24), slice(12340, 12364), slice(t - 24, t)):
+        want, off = _oracle(x.detach()[rows], w_gu, w_down, dy[rows], "silu")
+        assert ((y.detach()[rows].double() - want[0]).abs() <= off[0]).all() and ((dx[rows].double() - want[1]).abs() <= off[1]).all()

@@ -302,3 +302,11 @@ def test_a_few_tokens_quantised_inside_the_product(m, n, k):
     x[m // 2, k // 2] = float("nan")
     got, want = mx4_gemm(x, w), mx4_gemm(quantize_mx4(x), w)
     assert got[m // 2].isnan().all() and torch.equal(got.nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))
+
+
+def test_a_product_of_more_than_2_to_the_31_values():
+    from purlin_b200.ops.mx4 import mx4_gemm, quantize_mx4
+    x, w = _rand(70001, 64, 40), quantize_mx4(_rand(32776, 64, 41))
+    y = mx4_gemm(x, w)
+    for r in (0, 65530, 70001 - 300):
+        assert torch.equal(y[r:r + 300], mx4_gemm(x[r:r + 300].clone(), w))
