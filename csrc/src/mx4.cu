@@ -368,6 +368,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4WideKernel(const __grid_co
       for (int it = pairIdx; it < p.items && ok; it += numPairs, ++use) {
         const WideItem w = wideItem(p, it);
         const uint32_t shift = uint32_t(w.col0 % kScaleRows / 32);
+        const bool twoBlocks = w.col0 % kScaleRows + w.cols > kScaleRows;
         const uint32_t idesc = instrDescMx4(uint32_t(w.cols), 2 * kBM, 0), idescHigh = instrDescMx4(uint32_t(w.cols), 2 * kBM, 1);
         ok = waitAll(tmemEmpty, (use & 1) ^ 1, abortWord, p.timeoutNs);
         if (!ok) { if (elected) skinny::recordTimeout(p.status, 2, it, 0); break; }
@@ -377,16 +378,18 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4WideKernel(const __grid_co
           tc::fenceAfterThreadSync();
           const uint64_t off = uint64_t(st * (kWideStage >> 4)), da = descA0 + off, db = descB0 + off, ds = descS0 + off;
           const uint32_t scaleA = tmemBase + kScaleTmem + set * kScaleSet, scaleB = scaleA + 8;
-          // [scales of A: two blocks][of the first 128 columns: two blocks][of the next 128], 512 bytes each
+          // In the stage: [scales of A: two blocks][of the first 128 columns: two blocks][of the next 128], 512 bytes each. The copies that a half of
+          // the k-block needs come right before its MMAs, and columns that lie in one row block need no second copy: with few columns the
+          // copies take as long as the MMAs (us, all copies first / so: 256 x 4096 x 14336 18.1 / 16.8, 256 x 8192 x 8192 13.0 / 12.1).
 #pragma unroll
           for (uint32_t q = 0; q < 2; ++q) {
             scalesToTmem<2>(elected, scaleA + 4 * q, ds + 32 * q);
             scalesToTmem<2>(elected, scaleB + 8 * q, ds + 64 + 32 * q);
-            scalesToTmem<2>(elected, scaleB + 8 * q + 4, ds + 128 + 32 * q);
-          }
+            if (twoBlocks) scalesToTmem<2>(elected, scaleB + 8 * q + 4, ds + 128 + 32 * q);
 #pragma unroll
-          for (uint32_t k = 0; k < 4; ++k)      // (past K values and scales are zeros)
-            mmaMx4<2>(elected, tmemBase, da + 2 * k, db + 2 * k, k & 1 ? idescHigh : idesc, scaleA + 4 * (k / 2), scaleB + 8 * (k / 2) + shift, uint32_t(kb != 0 || k != 0));
+            for (uint32_t k = 2 * q; k < 2 * q + 2; ++k)      // (past K values and scales are zeros)
+              mmaMx4<2>(elected, tmemBase, da + 2 * k, db + 2 * k, k & 1 ? idescHigh : idesc, scaleA + 4 * q, scaleB + 8 * q + shift, uint32_t(kb != 0 || k != 0));
+          }
           commit<2>(elected, emptyBar(st));
           if (++st == kWideStages) { st = 0; ph ^= 1; }
         }
@@ -805,9 +808,10 @@ bool productFits(int M, int N, int K, int epilogue) {
 // whether the product quantises its activations itself
 bool quantisedInside(int dtype, int M) { return dtype == PURLIN_MX4_BF16 && M <= kDenseTokens; }
 
-// Rows of A up to which the kernel for few rows is taken (it has room for 128). The other one does not care how many of 256 there are, us, few rows 64 /
-// few rows 128 / the other: N, K 2048, 2048 5.7 / 7.2 / 6.3; 4096, 14336 13.5 / 19.8 / 17.7; 8192, 8192 11.6 / 15.7 / 12.4; 14336, 2048 gated 8.5 / 11.5 / 8.2.
-int fewRows(int N) { return N < 8192 ? 96 : 64; }
+// Rows of A up to which the kernel for few rows is taken (it has room for 128). The other one does not care how many of 256 there are; us, few rows 64 /
+// few rows 96 / the other: N, K 1024, 7168 6.3 / 7.3 / 9.1; 2048, 2048 5.1 / 5.6 / 5.1; 4096, 14336 13.3 / 17.1 / 15.2; 8192, 8192 few rows 64 11.3,
+// the other 10.9; 14336, 2048 7.4 and 7.5; 28672, 4096 11.2 and 14.4.
+int fewRows(int N) { return N < 8192 ? 80 : 64; }
 
 int launchWide(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, bool swiglu, uint32_t* status, const Device& dev,
                cudaStream_t stream) {
