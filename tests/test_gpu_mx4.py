@@ -121,7 +121,7 @@ def test_few_rows(m, n, k):
     _check_product(mx4_gemm(a, w), a, w, False)
 
 
-@pytest.mark.parametrize("m,n,k", [(129, 8, 32), (129, 264, 96), (256, 256, 256), (257, 128, 64), (300, 520, 544), (511, 1000, 288), (1000, 1024, 1120), (513, 14336, 256), (2049, 4104, 96), (200, 14208, 256), (500, 7104, 288),
+@pytest.mark.parametrize("m,n,k", [(129, 8, 32), (129, 264, 96), (256, 256, 256), (257, 128, 64), (300, 520, 544), (511, 1000, 288), (1000, 1024, 1120), (513, 14336, 256), (2049, 4104, 96), (200, 14208, 256), (500, 7104, 288), (1000, 14336, 96), (4096, 4864, 160),
                                     (4096, 2048, 2048)])
 def test_many_rows(m, n, k):
     from purlin_b200.ops.mx4 import mx4_gemm, quantize_mx4
@@ -129,7 +129,7 @@ def test_many_rows(m, n, k):
     _check_product(mx4_gemm(a, w), a, w, False)
 
 
-@pytest.mark.parametrize("m,i,k", [(1, 16, 32), (1, 3584, 1024), (7, 80, 96), (100, 528, 544), (128, 1024, 512), (129, 16, 64), (300, 528, 224), (1000, 1040, 512), (777, 7168, 256), (200, 7104, 256)])
+@pytest.mark.parametrize("m,i,k", [(1, 16, 32), (1, 3584, 1024), (7, 80, 96), (100, 528, 544), (128, 1024, 512), (129, 16, 64), (300, 528, 224), (1000, 1040, 512), (777, 7168, 256), (200, 7104, 256), (1000, 7168, 96)])      # the last ones: widths of 192 columns, tiles of the last wave in quarters
 def test_gated_product(m, i, k):
     from purlin_b200.ops.mx4 import mx4_gemm_swiglu, quantize_mx4
     a, w = quantize_mx4(_rand(m, k, 5)), quantize_mx4(_rand(2 * i, k, 6) * (4 * k ** -0.5))
