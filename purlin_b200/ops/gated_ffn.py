@@ -45,9 +45,9 @@ def gated_ffn(x: torch.Tensor, w_gu: torch.Tensor, w_down: torch.Tensor, activat
     """``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T`` for bf16 ``x [..., hidden]``, ``w_gu = interleave_gate_up(w_gate, w_up)``
     ``[2 * intermediate, hidden]`` and ``w_down [hidden, intermediate]``; differentiable once. ``activation``: "silu" or "gelu" (the form
     with the tanh). Where no gradient is asked for, nothing is kept. All tensors contiguous and on one device; hidden a multiple of 8,
-    intermediate of 16; any number of tokens, none included. The backward pass can be captured into a CUDA graph (after a first
-    pass outside of it); there use ``torch.autograd.grad``, because ``backward()`` accumulates on the stream on which an earlier graph of the same
-    leaves, if it is still alive, was made."""
+    intermediate of 16; any number of tokens, none included. Forward and backward can be captured into a
+    CUDA graph; there use ``torch.autograd.grad``, because ``backward()`` accumulates on the stream on which an earlier graph of the same leaves,
+    if it is still alive, was made."""
     _check(x, w_gu, w_down, activation)
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     y = _native.torch_ops().gated_ffn(rows, w_gu, w_down, ACTIVATIONS[activation])
