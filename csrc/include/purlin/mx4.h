@@ -24,11 +24,13 @@ int purlin_mx4_quantize(const void* x, int dtype, void* data, void* scales, int 
 int purlin_mx4_dequantize(const void* data, const void* scales, void* out, int dtype, int rows, int cols, void* stream);
 
 /* C[M, N] = A[M, K] * W[N, K]^T, fp32 accumulation, bf16 output; A and W as above. epilogue: PURLIN_EPI_STORE or PURLIN_EPI_SWIGLU (W's rows
- * alternate 16 of gate and 16 of up, N a multiple of 32, C is [M, N / 2]). N a multiple of 8. status: as in purlin_gemm_bf16. */
+ * alternate 16 of gate and 16 of up, N a multiple of 32, C is [M, N / 2]). N a multiple of 8. C overlaps no operand. status: as in
+ * purlin_gemm_bf16. */
 int purlin_mx4_gemm(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue,
                     uint32_t* status, void* stream);
 /* The same with activations x [M, K] of `dtype`, quantised by the way: a few tokens inside the product, more into the workspace first, which has
- * purlin_mx4_workspace_bytes() (none: it may be NULL). */
+ * purlin_mx4_workspace_bytes() (none: it may be NULL). C may overlap x, but neither w nor the workspace; a few tokens then take a workspace too,
+ * of M * K / 2 + purlin_mx4_scale_bytes(M, K) bytes. */
 size_t purlin_mx4_workspace_bytes(int dtype, int M, int K);
 int purlin_mx4_linear(const void* x, int dtype, void* workspace, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue,
                       uint32_t* status, void* stream);

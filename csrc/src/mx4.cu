@@ -805,6 +805,17 @@ bool productFits(int M, int N, int K, int epilogue) {
   if (int64_t(M) * N / 4096 > INT32_MAX / 4 || scaleBytes(std::max(M, N), K) / 128 > size_t(INT32_MAX)) { setError("mx4: the product is too large"); return false; }   // tile numbers, TMA coordinates
   return true;
 }
+bool overlap(const void* a, size_t aBytes, const void* b, size_t bBytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + bBytes && y < x + aBytes;
+}
+size_t productBytes(int M, int N, int epilogue) { return size_t(M) * size_t(epilogue == PURLIN_EPI_SWIGLU ? N / 2 : N) * 2; }
+// Tiles of C are stored while others still read their operands.
+bool apartFromOutput(const void* data, const void* scales, int rows, int cols, const void* C, size_t bytes) {
+  if (!overlap(data, size_t(rows) * size_t(cols) / 2, C, bytes) && !overlap(scales, scaleBytes(rows, cols), C, bytes)) return true;
+  setError("mx4: C overlaps a quantised operand");
+  return false;
+}
 // whether the product quantises its activations itself
 bool quantisedInside(int dtype, int M) { return dtype == PURLIN_MX4_BF16 && M <= kDenseTokens; }
 
@@ -909,6 +920,8 @@ int purlin_mx4_gemm(const void* aData, const void* aScales, const void* wData, c
   Device dev;
   if (!productFits(M, N, K, epilogue)) return 1;
   if (!aData || !aScales || !wData || !wScales || !C) { setError("mx4: an operand is missing"); return 1; }
+  const size_t bytes = productBytes(M, N, epilogue);
+  if (!apartFromOutput(aData, aScales, M, K, C, bytes) || !apartFromOutput(wData, wScales, N, K, C, bytes)) return 1;
   if (!currentDevice(dev)) return 1;
   return M <= fewRows(N) ? launchFew(nullptr, aData, aScales, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream))
                          : launchWide(aData, aScales, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream));
@@ -920,17 +933,21 @@ size_t purlin_mx4_workspace_bytes(int dtype, int M, int K) {
 
 int purlin_mx4_linear(const void* x, int dtype, void* workspace, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue, uint32_t* status, void* stream) {
   if (!productFits(M, N, K, epilogue)) return 1;
-  if (quantisedInside(dtype, M)) {
+  // Where C overlaps x, x is quantised by a launch of its own first: inside the product CTAs that are done would write over what others still read.
+  const size_t bytes = productBytes(M, N, epilogue);
+  const bool overX = overlap(x, size_t(M) * size_t(K) * (dtype == PURLIN_MX4_FP32 ? 4 : 2), C, bytes);
+  if (quantisedInside(dtype, M) && !overX) {
     const bool swiglu = epilogue == PURLIN_EPI_SWIGLU;
     NvtxRange range(swiglu ? "mx4LinearSwiglu" : "mx4Linear", size_t(M) * size_t(N) * 2);
     Device dev;
     if (!x || !wData || !wScales || !C) { setError("mx4: an operand is missing"); return 1; }
     if (reinterpret_cast<uintptr_t>(x) % 16) { setError("mx4: tensors must start on a 16-byte boundary"); return 1; }
+    if (!apartFromOutput(wData, wScales, N, K, C, bytes)) return 1;
     if (!currentDevice(dev)) return 1;
     return launchFew(x, nullptr, nullptr, wData, wScales, C, M, N, K, swiglu, status, dev, static_cast<cudaStream_t>(stream));
   }
   unsigned char* data = static_cast<unsigned char*>(workspace);
-  if (!data) { setError("mx4: an operand is missing"); return 1; }
+  if (!data) { setError(overX ? "mx4: C overlaps x, which takes a workspace" : "mx4: an operand is missing"); return 1; }
   unsigned char* scales = data + size_t(M) * size_t(K) / 2;       // (a row is a multiple of 16 bytes)
   const int rc = purlin_mx4_quantize(x, dtype, data, scales, M, K, stream);
   return rc ? rc : purlin_mx4_gemm(data, scales, wData, wScales, C, M, N, K, epilogue, status, stream);

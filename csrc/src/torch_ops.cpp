@@ -108,15 +108,23 @@ Tensor dequantize(const Tensor& data, const Tensor& scales, int64_t type) {
   return out;
 }
 
+bool overlap(const Tensor& a, const Tensor& b) {
+  const auto x = reinterpret_cast<uintptr_t>(a.data_ptr()), y = reinterpret_cast<uintptr_t>(b.data_ptr());
+  return x < y + b.nbytes() && y < x + a.nbytes();
+}
+
 // out[rows of a, N or N / 2]; `a` is dense of type `type`, or quantised with its scales
 void product(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales, const Tensor& wData, const Tensor& wScales, const Tensor& out, int64_t rows, int64_t epilogue) {
   const c10::cuda::CUDAGuard guard(wData.device());
   const int64_t n = wData.size(0), k = 2 * wData.size(1);
+  if (overlap(out, wData) || overlap(out, wScales) || (aScales && (overlap(out, a) || overlap(out, *aScales)))) throw std::invalid_argument("out overlaps a quantised operand");
   if (aScales) {
     check(purlin_mx4_gemm(a.data_ptr(), aScales->data_ptr(), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), int(rows), int(n), int(k), int(epilogue), nullptr, stream()));
   } else {
     Tensor work;
-    if (const size_t size = purlin_mx4_workspace_bytes(int(type), int(rows), int(k))) work = bytes(int64_t(size), wData);
+    size_t size = purlin_mx4_workspace_bytes(int(type), int(rows), int(k));
+    if (!size && overlap(out, a)) size = size_t(rows) * size_t(k) / 2 + purlin_mx4_scale_bytes(int(rows), int(k));
+    if (size) work = bytes(int64_t(size), wData);
     check(purlin_mx4_linear(a.data_ptr(), int(type), ptr(work), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), int(rows), int(n), int(k), int(epilogue), nullptr, stream()));
   }
 }

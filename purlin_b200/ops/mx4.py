@@ -116,10 +116,10 @@ def _product(a: Union[torch.Tensor, Mx4Tensor], w: Mx4Tensor, out: Optional[torc
 
 def mx4_gemm(a: Union[torch.Tensor, Mx4Tensor], w: Mx4Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a @ w.T`` in bf16 for ``a [..., K]``, an ``Mx4Tensor`` or a bf16, fp16 or fp32 tensor that is quantised in the call, and ``w [N, K]``; N a multiple of
-    8. One token or many."""
+    8. One token or many. ``out`` may be (or overlap) a dense ``a``; it may not overlap a quantised operand."""
     return _product(a, w, out, EPI_STORE)
 
 
 def mx4_gemm_swiglu(a: Union[torch.Tensor, Mx4Tensor], w_gu: Mx4Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``silu(a @ w_gate.T) * (a @ w_up.T)`` for ``w_gu = quantize_mx4(interleave_gate_up(w_gate, w_up))``."""
+    """``silu(a @ w_gate.T) * (a @ w_up.T)`` for ``w_gu = quantize_mx4(interleave_gate_up(w_gate, w_up))``; ``a`` and ``out`` as in ``mx4_gemm``."""
     return _product(a, w_gu, out, EPI_SWIGLU)

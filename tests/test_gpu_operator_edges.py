@@ -1,0 +1,44 @@
+"""The operators of the gated block at the edges of what their documentation allows."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _rand(rows, cols, seed, dtype=torch.bfloat16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(rows, cols, generator=g, device="cuda").to(dtype)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 64, 65, 300])
+def test_a_product_in_place_of_its_activations(m):
+    # on both sides of every border between the kernels: the output is the activations' own memory, all of it or a part
+    from purlin_b200.ops.mx4 import mx4_gemm, mx4_gemm_swiglu, quantize_mx4
+    k = 8192 if m < 5 else 1024
+    x, w = _rand(m, k, m), quantize_mx4(_rand(k, k, 1))
+    want, gated = mx4_gemm(x, w), mx4_gemm_swiglu(x, w)
+    for _ in range(3):
+        y = x.clone()
+        assert mx4_gemm(y, w, out=y) is y and torch.equal(y, want)
+        y = x.clone()
+        half = y.flatten()[:m * k // 2].view(m, k // 2)
+        assert torch.equal(mx4_gemm_swiglu(y, w, out=half), gated)
+        room = torch.zeros(m * k + 64, dtype=torch.bfloat16, device="cuda")
+        room[:m * k] = x.flatten()
+        assert torch.equal(mx4_gemm(room[:m * k].view(m, k), w, out=room[64:].view(m, k)), want) and torch.equal(room[:64], x.flatten()[:64])
+
+
+@pytest.mark.parametrize("m", [2, 300])
+def test_a_product_over_a_quantised_operand_is_refused(m):
+    from purlin_b200.ops.mx4 import Mx4Tensor, mx4_gemm, quantize_mx4
+    x = _rand(m, 256, 1)
+    room = torch.zeros(m * 256 * 2 + 2 ** 16, dtype=torch.uint8, device="cuda")
+    out = room[:m * 512].view(torch.bfloat16).view(m, 256)
+    q, w = quantize_mx4(x), quantize_mx4(_rand(256, 256, 2))
+    inside = Mx4Tensor(room[:m * 128].view(m, 128), q.scales)
+    with pytest.raises(ValueError, match="overlaps"):
+        mx4_gemm(inside, w, out=out)
+    tail = Mx4Tensor(w.data, room[m * 512 - 16:][:w.scales.numel()])
+    for a in (x, q):
+        with pytest.raises(ValueError, match="overlaps"):
+            mx4_gemm(a, tail, out=out)

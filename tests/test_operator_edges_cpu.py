@@ -1,0 +1,28 @@
+"""What the operators of the gated block refuse, or have to have in their source, at the edges of what they take; no GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+i, p, n = C.c_int, C.c_void_p, None
+
+
+def _refusal(rc):
+    from purlin_b200 import _native
+    assert rc != 0
+    return _native.last_error(_native.cuda())
+
+
+def test_products_refuse_an_output_over_their_operands():
+    # addresses that no call follows: the refusal comes before anything is launched
+    from purlin_b200 import _native
+    lib = _native.cuda()
+    a, sa, w, sw, c = (p(v << 20) for v in range(1, 6))
+    m, cols, k = 4, 64, 64
+    for at in ((1 << 20) + 32, (2 << 20) + 496, (3 << 20) + 2032, (4 << 20), (1 << 20) - 496, (3 << 20) - 496):     # C: 512 bytes; a 128, w 2048, scales 512
+        assert "overlaps" in _refusal(lib.purlin_mx4_gemm(a, sa, w, sw, p(at), i(m), i(cols), i(k), i(0), n, n)), at
+        if at > 2.5 * 2 ** 20:
+            assert "overlaps" in _refusal(lib.purlin_mx4_linear(c, i(0), n, w, sw, p(at), i(m), i(cols), i(k), i(0), n, n)), at
+    # x itself: quantised by a launch of its own, for which there is no workspace here
+    for at in (5 << 20, (5 << 20) - 496, (5 << 20) + 496):
+        assert "overlaps x" in _refusal(lib.purlin_mx4_linear(c, i(0), n, w, sw, p(at), i(m), i(cols), i(k), i(0), n, n)), at
