@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffnKernel(const __grid_constant__
 // The parts of a product whose k was split, added in ascending order of k: a warp per 32 rows x 32 columns, a row to a lane, as the epilogue
 // laid them down. (A second launch and not the last part's epilogue: one warp adding up sixteen parts takes far longer than all.)
 constexpr int kFinishThreads = 256;
-__global__ void __launch_bounds__(kFinishThreads) finishKernel(const float4* __restrict__ partial, __nv_bfloat16* __restrict__ out, int M, int N, int split, int tiles, int tilesM, int tilesN,
+__global__ void __launch_bounds__(kFinishThreads) finishKernel(const float4* partial, __nv_bfloat16* out, int M, int N, int split, int tiles, int tilesM, int tilesN,
                                                                 int blocksM, int bn, int64_t warps) {
   tc::gridDependencyWait();
   tc::gridLaunchDependents();

@@ -40,9 +40,11 @@ constexpr int kScaleRows = 128, kScaleCols = 128, kScaleBytes = 512;
 // the way back 24.8 us; 14336 x 8192 fp32 78.5 us, 6.8 TB/s; with one chain per block 8192 x 8192 took 104 us there and back.
 constexpr int kVec = 8, kWarpCols = 32 * kVec, kQuantThreads = 256, kUnroll = 4, kStepCols = kUnroll * kWarpCols;
 
+// Not through the non-coherent path, and no pointer of these kernels promises it (const, restrict): that path is for memory that nobody writes during a
+// kernel's whole life, and these kernels are set up while the one before them may still write what they will read.
 PURLIN_D uint4 ldOnce(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 
@@ -105,8 +107,7 @@ PURLIN_D size_t scaleOffset(int row, int col, int colBlocks) {       // of the s
 
 // Rows past the last one (up to the scales' 128) write their zeros.
 template <int TYPE>
-__global__ void __launch_bounds__(kQuantThreads) quantizeKernel(const unsigned char* __restrict__ x, unsigned char* __restrict__ data, unsigned char* __restrict__ scales,
-                                                                int rows, int cols, uint32_t steps, uint32_t total) {
+__global__ void __launch_bounds__(kQuantThreads) quantizeKernel(const unsigned char* x, unsigned char* data, unsigned char* scales, int rows, int cols, uint32_t steps, uint32_t total) {
   tc::gridDependencyWait();
   tc::gridLaunchDependents();
   constexpr int kSize = TYPE == PURLIN_MX4_FP32 ? 4 : 2;
@@ -157,8 +158,7 @@ PURLIN_D float powerOf(uint32_t scale) {      // 2^(scale - 127); 2^-127 is belo
 }
 
 template <int TYPE>
-__global__ void __launch_bounds__(kQuantThreads) dequantizeKernel(const unsigned char* __restrict__ data, const unsigned char* __restrict__ scales, unsigned char* __restrict__ out,
-                                                                  int rows, int cols, uint32_t steps, uint32_t total) {
+__global__ void __launch_bounds__(kQuantThreads) dequantizeKernel(const unsigned char* data, const unsigned char* scales, unsigned char* out, int rows, int cols, uint32_t steps, uint32_t total) {
   tc::gridDependencyWait();
   tc::gridLaunchDependents();
   const int lane = threadIdx.x & 31;

@@ -42,3 +42,37 @@ def test_a_product_over_a_quantised_operand_is_refused(m):
     for a in (x, q):
         with pytest.raises(ValueError, match="overlaps"):
             mx4_gemm(a, tail, out=out)
+
+
+def test_producer_quantisation_and_the_way_back_over_the_same_buffers():
+    # each kernel is set up while the one before it writes what it will read; the values change from pass to pass, the buffers stay, in a graph too
+    from purlin_b200.ops.mx4 import mx4_gemm_swiglu, quantize_mx4
+    w = quantize_mx4(_rand(2 * 2048, 256, 3))
+    x, h = torch.empty(700, 256, dtype=torch.bfloat16, device="cuda"), torch.empty(700, 2048, dtype=torch.bfloat16, device="cuda")
+
+    def work():
+        mx4_gemm_swiglu(x, w, out=h)
+        return quantize_mx4(h).dequantize()
+
+    news = [_rand(700, 256, 50 + n) for n in range(8)]
+    wants = []
+    for new in news:                                # one kernel at a time
+        f = mx4_gemm_swiglu(new, w)
+        torch.cuda.synchronize()
+        q = quantize_mx4(f)
+        torch.cuda.synchronize()
+        wants.append(q.dequantize())
+        torch.cuda.synchronize()
+    x.copy_(news[0])
+    work()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    got = []
+    for _ in range(5):
+        for new in news:
+            x.copy_(new)
+            got.append(work())
+            graph.replay()
+            got.append(out.clone())
+    assert all(torch.equal(v, wants[n // 2 % 8]) for n, v in enumerate(got))

@@ -26,3 +26,17 @@ def test_products_refuse_an_output_over_their_operands():
     # x itself: quantised by a launch of its own, for which there is no workspace here
     for at in (5 << 20, (5 << 20) - 496, (5 << 20) + 496):
         assert "overlaps x" in _refusal(lib.purlin_mx4_linear(c, i(0), n, w, sw, p(at), i(m), i(cols), i(k), i(0), n, n)), at
+
+
+def test_no_load_of_the_kernels_takes_the_non_coherent_path():
+    # Kernels here are set up while the one before them still runs, and wait for it inside. The non-coherent path is defined for memory that nobody
+    # writes during a kernel's whole life, set-up included; no run shows a stale line reliably, so the source is read: no such load, and no
+    # kernel's pointer that is const and restrict, which lets the compiler choose one.
+    import re
+    from pathlib import Path
+    csrc = Path(__file__).resolve().parent.parent / "csrc"
+    for path in sorted([*csrc.glob("src/*.cu"), *csrc.glob("include/purlin/*.cuh")]):
+        text = path.read_text()
+        assert not re.search(r"\bld\.global[\w.:]*\.nc\b|__ldg\(", text), path.name
+        for head in re.findall(r"__global__[^{;]*", text):
+            assert not re.search(r"\bconst\s+[\w:]+\s*\*\s*__restrict__", head), (path.name, head[:200])
