@@ -24,6 +24,10 @@ using torch::autograd::variable_list;
 void check(int rc) {
   if (rc) throw std::runtime_error(std::string("purlin: ") + purlin_last_error());
 }
+int narrow(int64_t v) {      // of a size that the C entries count in 32 bits
+  if (v < 0 || v > INT32_MAX) throw std::invalid_argument("a dimension of 2^31 or more");
+  return int(v);
+}
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
@@ -95,8 +99,8 @@ Tensor gatedFfn(const Tensor& x, const Tensor& wGateUp, const Tensor& wDown, int
 
 std::tuple<Tensor, Tensor> quantize(const Tensor& x, int64_t type, int64_t rows, int64_t cols) {
   const c10::cuda::CUDAGuard guard(x.device());
-  Tensor data = at::empty({rows, cols / 2}, x.options().dtype(at::kByte)), scales = bytes(int64_t(purlin_mx4_scale_bytes(int(rows), int(cols))), x);
-  if (rows) check(purlin_mx4_quantize(x.data_ptr(), int(type), data.data_ptr(), scales.data_ptr(), int(rows), int(cols), stream()));
+  Tensor data = at::empty({rows, cols / 2}, x.options().dtype(at::kByte)), scales = bytes(int64_t(purlin_mx4_scale_bytes(narrow(rows), narrow(cols))), x);
+  if (rows) check(purlin_mx4_quantize(x.data_ptr(), int(type), data.data_ptr(), scales.data_ptr(), narrow(rows), narrow(cols), stream()));
   return {data, scales};
 }
 
@@ -104,7 +108,7 @@ Tensor dequantize(const Tensor& data, const Tensor& scales, int64_t type) {
   const c10::cuda::CUDAGuard guard(data.device());
   const int64_t rows = data.size(0), cols = 2 * data.size(1);
   Tensor out = at::empty({rows, cols}, data.options().dtype(type == PURLIN_MX4_FP32 ? at::kFloat : at::kBFloat16));
-  if (rows) check(purlin_mx4_dequantize(data.data_ptr(), scales.data_ptr(), out.data_ptr(), int(type), int(rows), int(cols), stream()));
+  if (rows) check(purlin_mx4_dequantize(data.data_ptr(), scales.data_ptr(), out.data_ptr(), int(type), narrow(rows), narrow(cols), stream()));
   return out;
 }
 
@@ -119,13 +123,13 @@ void product(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales
   const int64_t n = wData.size(0), k = 2 * wData.size(1);
   if (overlap(out, wData) || overlap(out, wScales) || (aScales && (overlap(out, a) || overlap(out, *aScales)))) throw std::invalid_argument("out overlaps a quantised operand");
   if (aScales) {
-    check(purlin_mx4_gemm(a.data_ptr(), aScales->data_ptr(), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), int(rows), int(n), int(k), int(epilogue), nullptr, stream()));
+    check(purlin_mx4_gemm(a.data_ptr(), aScales->data_ptr(), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), narrow(rows), narrow(n), narrow(k), int(epilogue), nullptr, stream()));
   } else {
     Tensor work;
-    size_t size = purlin_mx4_workspace_bytes(int(type), int(rows), int(k));
-    if (!size && overlap(out, a)) size = size_t(rows) * size_t(k) / 2 + purlin_mx4_scale_bytes(int(rows), int(k));
+    size_t size = purlin_mx4_workspace_bytes(int(type), narrow(rows), narrow(k));
+    if (!size && overlap(out, a)) size = size_t(rows) * size_t(k) / 2 + purlin_mx4_scale_bytes(narrow(rows), narrow(k));
     if (size) work = bytes(int64_t(size), wData);
-    check(purlin_mx4_linear(a.data_ptr(), int(type), ptr(work), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), int(rows), int(n), int(k), int(epilogue), nullptr, stream()));
+    check(purlin_mx4_linear(a.data_ptr(), int(type), ptr(work), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), narrow(rows), narrow(n), narrow(k), int(epilogue), nullptr, stream()));
   }
 }
 Tensor newProduct(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales, const Tensor& wData, const Tensor& wScales, std::vector<int64_t> shape, int64_t rows,

@@ -14,12 +14,20 @@ from .. import _native
 
 EPI_STORE, EPI_SWIGLU = 0, 1
 MAX_ROWS = 2 ** 30
+MAX_COLS = 2 ** 31 - 1056        # a step of the quantisation past them still counts in 32 bits
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def scale_bytes(rows: int, cols: int) -> int:
     """Bytes of the scales of a [rows, cols] tensor: 512 for every 128 rows x 128 columns, the last ones filled up."""
     return -(-rows // 128) * -(-cols // 128) * 512
+
+
+def _check_sizes(rows: int, cols: int):
+    if rows > MAX_ROWS:
+        raise ValueError("at most 2^30 rows")
+    if cols > MAX_COLS:
+        raise ValueError("at most 2^31 - 1056 columns")
 
 
 class Mx4Tensor:
@@ -33,12 +41,11 @@ class Mx4Tensor:
             raise TypeError("data and scales are uint8 tensors")
         if data.dim() != 2 or data.shape[1] == 0 or data.shape[1] % 16 or scales.numel() != scale_bytes(data.shape[0], 2 * data.shape[1]):
             raise ValueError("data is [rows, cols / 2] with cols a multiple of 32, and scales has 512 bytes for every 128 rows x 128 columns")
+        _check_sizes(data.shape[0], 2 * data.shape[1])
         if not (data.is_cuda and scales.device == data.device and data.is_contiguous() and scales.is_contiguous()):
             raise ValueError("data and scales must be contiguous CUDA tensors on one device")
         if (data.data_ptr() | scales.data_ptr()) % 16:
             raise ValueError("data and scales must start on a 16-byte boundary")
-        if data.shape[0] > MAX_ROWS:
-            raise ValueError("at most 2^30 rows")
         self.data, self.scales, self.shape, self.device = data, scales, (data.shape[0], 2 * data.shape[1]), data.device
 
     @classmethod
@@ -69,13 +76,12 @@ def _check_dense(x: torch.Tensor) -> Tuple[int, int, int]:
     cols = shape[-1] if shape else 0
     if cols == 0 or cols % 32:
         raise ValueError("the last dimension must be a multiple of 32")
+    rows = x.numel() // cols
+    _check_sizes(rows, cols)
     if not (x.is_cuda and x.is_contiguous()):
         raise ValueError("operands must be contiguous CUDA tensors")
     if x.data_ptr() % 16:
         raise ValueError("operands must start on a 16-byte boundary")
-    rows = x.numel() // cols
-    if rows > MAX_ROWS:
-        raise ValueError("at most 2^30 rows")
     return rows, cols, kind
 
 

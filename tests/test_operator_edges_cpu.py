@@ -40,3 +40,23 @@ def test_no_load_of_the_kernels_takes_the_non_coherent_path():
         assert not re.search(r"\bld\.global[\w.:]*\.nc\b|__ldg\(", text), path.name
         for head in re.findall(r"__global__[^{;]*", text):
             assert not re.search(r"\bconst\s+[\w:]+\s*\*\s*__restrict__", head), (path.name, head[:200])
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+def test_rows_of_2_to_the_31_values_are_refused():
+    # the kernels count columns in 32 bits; 2^32 + 64 of them would be 64
+    from purlin_b200 import _native
+    from purlin_b200.ops.mx4 import Mx4Tensor, mx4_gemm, quantize_mx4, scale_bytes
+    for cols in (2 ** 31 - 1024, 2 ** 31, 2 ** 32 + 64):
+        for dtype in (torch.bfloat16, torch.float16, torch.float32):
+            with pytest.raises(ValueError, match="columns"):
+                quantize_mx4(_meta(1, cols, dtype=dtype))
+        with pytest.raises(ValueError, match="columns"):
+            Mx4Tensor(_meta(1, cols // 2, dtype=torch.uint8), _meta(scale_bytes(1, cols), dtype=torch.uint8))
+    with pytest.raises(ValueError, match="CUDA"):               # the widest that fits: refused for its device alone
+        quantize_mx4(_meta(1, 2 ** 31 - 1056))
+    lib = _native.cuda()
+    assert "large" in _refusal(lib.purlin_mx4_quantize(p(4096), i(0), p(4096), p(4096), i(1), i(2 ** 31 - 1024), n))
