@@ -634,7 +634,7 @@ int gradients(Product (&g)[kMaxGroups], const void* x, const void* wGateUp, cons
 bool sizesFit(int tokens, int hidden, int intermediate, int activation) {
   if (tokens <= 0 || hidden <= 0 || intermediate <= 0) { setError("feed-forward: dimensions must be positive"); return false; }
   if (hidden % 8 || intermediate % 16) { setError("feed-forward: hidden must be a multiple of 8 and intermediate of 16"); return false; }
-  if (intermediate > INT32_MAX / 4 || hidden > INT32_MAX / 4 || tokens > INT32_MAX / 4) { setError("feed-forward: dimensions above 2^29"); return false; }
+  if (intermediate > INT32_MAX / 4 || hidden > INT32_MAX / 4 || tokens > INT32_MAX / 4) { setError("feed-forward: dimensions must be below 2^29"); return false; }
   if (activation != PURLIN_ACT_SILU && activation != PURLIN_ACT_GELU) { setError("feed-forward: unknown activation"); return false; }
   return true;
 }

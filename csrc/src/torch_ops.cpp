@@ -37,9 +37,9 @@ std::tuple<Tensor, Tensor, Tensor> ffnForward(const Tensor& x, const Tensor& wGa
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t tokens = x.size(0), hidden = wDown.size(0), intermediate = wDown.size(1);
   Tensor y = at::empty_like(x), h = at::empty({tokens, intermediate}, x.options()), saved;
-  if (keep) saved = bytes(int64_t(purlin_ffn_saved_bytes(int(tokens), int(intermediate))), x);
+  if (keep) saved = bytes(int64_t(purlin_ffn_saved_bytes(narrow(tokens), narrow(intermediate))), x);
   if (tokens)
-    check(purlin_ffn_forward(x.data_ptr(), wGateUp.data_ptr(), wDown.data_ptr(), h.data_ptr(), ptr(saved), y.data_ptr(), int(tokens), int(hidden), int(intermediate),
+    check(purlin_ffn_forward(x.data_ptr(), wGateUp.data_ptr(), wDown.data_ptr(), h.data_ptr(), ptr(saved), y.data_ptr(), narrow(tokens), narrow(hidden), narrow(intermediate),
                              int(activation), nullptr, stream()));
   return {y, h, saved};
 }
@@ -77,9 +77,9 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
         if (reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16) dy = dy.clone();
         if (needs & 3) dz = at::empty({tokens, 2 * intermediate}, x.options());
         Tensor work;
-        if (const size_t n = purlin_ffn_workspace_bytes(int(tokens), int(hidden), int(intermediate), int(needs & 1), int(needs & 2), int(needs & 4))) work = bytes(int64_t(n), x);
+        if (const size_t n = purlin_ffn_workspace_bytes(narrow(tokens), narrow(hidden), narrow(intermediate), int(needs & 1), int(needs & 2), int(needs & 4))) work = bytes(int64_t(n), x);
         check(purlin_ffn_backward(x.data_ptr(), wGateUp.data_ptr(), wDown.data_ptr(), ptr(h), ptr(saved), dy.data_ptr(), ptr(dz), ptr(dx), ptr(dGateUp), ptr(dDown), ptr(work),
-                                  work.defined() ? size_t(work.numel()) : 0, int(tokens), int(hidden), int(intermediate), int(ctx->saved_data["activation"].toInt()), nullptr, stream()));
+                                  work.defined() ? size_t(work.numel()) : 0, narrow(tokens), narrow(hidden), narrow(intermediate), int(ctx->saved_data["activation"].toInt()), nullptr, stream()));
       }
     }
     variable_list out{dx, dGateUp, dDown};

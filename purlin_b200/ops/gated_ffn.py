@@ -31,8 +31,8 @@ def _check(x: torch.Tensor, w_gu: torch.Tensor, w_down: torch.Tensor, activation
         raise ValueError("x is [..., hidden], w_gu is [2 * intermediate, hidden] and w_down is [hidden, intermediate]")
     if hidden == 0 or intermediate == 0 or hidden % 8 or intermediate % 16:
         raise ValueError("hidden must be a multiple of 8 and intermediate of 16")
-    if x.numel() // hidden > 2 ** 29:
-        raise ValueError("at most 2^29 tokens")
+    if max(x.numel() // hidden, hidden, intermediate) >= 2 ** 29:
+        raise ValueError("tokens, hidden and intermediate must be below 2^29")
     if not (x.is_cuda and w_gu.device == x.device and w_down.device == x.device):
         raise ValueError("operands must be CUDA tensors on one device")
     if not (x.is_contiguous() and w_gu.is_contiguous() and w_down.is_contiguous()):
@@ -45,7 +45,7 @@ def gated_ffn(x: torch.Tensor, w_gu: torch.Tensor, w_down: torch.Tensor, activat
     """``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T`` for bf16 ``x [..., hidden]``, ``w_gu = interleave_gate_up(w_gate, w_up)``
     ``[2 * intermediate, hidden]`` and ``w_down [hidden, intermediate]``; differentiable once. ``activation``: "silu" or "gelu" (the form
     with the tanh). Where no gradient is asked for, nothing is kept. All tensors contiguous and on one device; hidden a multiple of 8,
-    intermediate of 16; any number of tokens, none included. Forward and backward can be captured into a
+    intermediate of 16; any number of tokens below 2^29, none included. Forward and backward can be captured into a
     CUDA graph; there use ``torch.autograd.grad``, because ``backward()`` accumulates on the stream on which an earlier graph of the same leaves,
     if it is still alive, was made."""
     _check(x, w_gu, w_down, activation)

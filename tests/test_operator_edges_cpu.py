@@ -60,3 +60,17 @@ def test_rows_of_2_to_the_31_values_are_refused():
         quantize_mx4(_meta(1, 2 ** 31 - 1056))
     lib = _native.cuda()
     assert "large" in _refusal(lib.purlin_mx4_quantize(p(4096), i(0), p(4096), p(4096), i(1), i(2 ** 31 - 1024), n))
+
+
+def test_the_block_refuses_2_to_the_29_tokens_in_python_as_in_c():
+    from purlin_b200 import _native
+    from purlin_b200.ops.gated_ffn import gated_ffn
+    most = 2 ** 29
+    for tokens, hidden, intermediate in ((most, 64, 32), (most + 5, 64, 32), (4, most, 16), (4, 8, most), (1, 2 ** 32 + 8, 16), (1, 8, 2 ** 32 + 16)):
+        with pytest.raises(ValueError, match=r"below 2\^29"):
+            gated_ffn(_meta(tokens, hidden), _meta(2 * intermediate, hidden), _meta(hidden, intermediate))
+    with pytest.raises(ValueError, match="CUDA"):
+        gated_ffn(_meta(most - 1, 64), _meta(64, 64), _meta(64, 32))
+    lib = _native.cuda()
+    for sizes in ((most, 64, 32), (4, most, 16), (4, 8, most)):
+        assert "below 2^29" in _refusal(lib.purlin_ffn_forward(p(4096), p(4096), p(4096), p(4096), n, p(4096), *map(i, sizes), i(0), n, n))
