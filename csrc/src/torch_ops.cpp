@@ -32,6 +32,12 @@ void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 
+// The tangent of a dual tensor (forward-mode differentiation) would be dropped without a word: the kernels see the values alone.
+void refuseTangents(const char* name, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    if (t->_fw_grad(/*level=*/0).defined()) throw std::runtime_error(std::string(name) + " has no forward-mode derivative");
+}
+
 // y and h, and the pre-activations where the backward will want them
 std::tuple<Tensor, Tensor, Tensor> ffnForward(const Tensor& x, const Tensor& wGateUp, const Tensor& wDown, int64_t activation, bool keep) {
   const c10::cuda::CUDAGuard guard(x.device());
@@ -62,6 +68,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
     const int64_t tokens = x.size(0), hidden = wDown.size(0), intermediate = wDown.size(1);
     Tensor dx, dGateUp, dDown, dz;
     if (!grads[0].defined()) return {dx, dGateUp, dDown, Tensor()};
+    refuseTangents("gated_ffn's backward pass", {&grads[0]});
     const bool again = at::GradMode::is_enabled() && (grads[0].requires_grad() || needs);
     {
       at::AutoGradMode off(false);
@@ -93,6 +100,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
 };
 
 Tensor gatedFfn(const Tensor& x, const Tensor& wGateUp, const Tensor& wDown, int64_t activation) {
+  refuseTangents("gated_ffn", {&x, &wGateUp, &wDown});
   if (at::GradMode::is_enabled() && (x.requires_grad() || wGateUp.requires_grad() || wDown.requires_grad())) return GatedFfn::apply(x, wGateUp, wDown, activation);
   return std::get<0>(ffnForward(x, wGateUp, wDown, activation, false));
 }

@@ -43,7 +43,7 @@ def _check(x: torch.Tensor, w_gu: torch.Tensor, w_down: torch.Tensor, activation
 
 def gated_ffn(x: torch.Tensor, w_gu: torch.Tensor, w_down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
     """``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T`` for bf16 ``x [..., hidden]``, ``w_gu = interleave_gate_up(w_gate, w_up)``
-    ``[2 * intermediate, hidden]`` and ``w_down [hidden, intermediate]``; differentiable once. ``activation``: "silu" or "gelu" (the form
+    ``[2 * intermediate, hidden]`` and ``w_down [hidden, intermediate]``; differentiable once, in reverse mode (a forward-mode derivative is refused). ``activation``: "silu" or "gelu" (the form
     with the tanh). Where no gradient is asked for, nothing is kept. All tensors contiguous and on one device; hidden a multiple of 8,
     intermediate of 16; any number of tokens below 2^29, none included. Forward and backward can be captured into a
     CUDA graph; there use ``torch.autograd.grad``, because ``backward()`` accumulates on the stream on which an earlier graph of the same leaves,

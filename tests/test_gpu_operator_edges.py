@@ -76,3 +76,20 @@ def test_producer_quantisation_and_the_way_back_over_the_same_buffers():
             graph.replay()
             got.append(out.clone())
     assert all(torch.equal(v, wants[n // 2 % 8]) for n, v in enumerate(got))
+
+
+def test_forward_mode_derivatives_of_the_block_are_refused():
+    from purlin_b200.ops.gated_ffn import gated_ffn
+    args = [_rand(16, 64, 1), _rand(64, 64, 2), _rand(64, 32, 3)]
+    with torch.autograd.forward_ad.dual_level():
+        for k in range(3):
+            called = list(args)
+            called[k] = torch.autograd.forward_ad.make_dual(args[k], torch.ones_like(args[k]))
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError, match="forward-mode"):
+                    gated_ffn(*called)
+        assert gated_ffn(*args).shape == (16, 64)            # a dual level alone is no reason
+        leaves = [v.clone().requires_grad_() for v in args]
+        y = gated_ffn(*leaves)
+        with pytest.raises(RuntimeError, match="forward-mode"):                                      # of the backward pass
+            torch.autograd.grad(y, leaves, torch.autograd.forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))

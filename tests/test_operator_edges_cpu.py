@@ -74,3 +74,22 @@ def test_the_block_refuses_2_to_the_29_tokens_in_python_as_in_c():
     lib = _native.cuda()
     for sizes in ((most, 64, 32), (4, most, 16), (4, 8, most)):
         assert "below 2^29" in _refusal(lib.purlin_ffn_forward(p(4096), p(4096), p(4096), p(4096), n, p(4096), *map(i, sizes), i(0), n, n))
+
+
+def _dual(t):
+    return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+
+def test_forward_mode_derivatives_are_refused():
+    # below the checks of the device, so that it needs none: a tangent on any argument, with and without gradients asked for
+    from purlin_b200 import _native
+    ops = _native.torch_ops()
+    args = [torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(64, 64, dtype=torch.bfloat16), torch.zeros(64, 32, dtype=torch.bfloat16)]
+    with torch.autograd.forward_ad.dual_level():
+        for k in range(3):
+            for needs in (False, True):
+                called = [v.clone().requires_grad_(needs) for v in args]
+                called[k] = _dual(called[k])
+                for mode in (torch.enable_grad, torch.no_grad):
+                    with mode(), pytest.raises(RuntimeError, match="forward-mode"):
+                        ops.gated_ffn(*called, 0)
