@@ -106,6 +106,7 @@ Tensor gatedFfn(const Tensor& x, const Tensor& wGateUp, const Tensor& wDown, int
 }
 
 std::tuple<Tensor, Tensor> quantize(const Tensor& x, int64_t type, int64_t rows, int64_t cols) {
+  refuseTangents("a 4-bit quantisation", {&x});
   const c10::cuda::CUDAGuard guard(x.device());
   Tensor data = at::empty({rows, cols / 2}, x.options().dtype(at::kByte)), scales = bytes(int64_t(purlin_mx4_scale_bytes(narrow(rows), narrow(cols))), x);
   if (rows) check(purlin_mx4_quantize(x.data_ptr(), int(type), data.data_ptr(), scales.data_ptr(), narrow(rows), narrow(cols), stream()));
@@ -126,7 +127,7 @@ bool overlap(const Tensor& a, const Tensor& b) {
 }
 
 // out[rows of a, N or N / 2]; `a` is dense of type `type`, or quantised with its scales
-void product(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales, const Tensor& wData, const Tensor& wScales, const Tensor& out, int64_t rows, int64_t epilogue) {
+void multiply(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales, const Tensor& wData, const Tensor& wScales, const Tensor& out, int64_t rows, int64_t epilogue) {
   const c10::cuda::CUDAGuard guard(wData.device());
   const int64_t n = wData.size(0), k = 2 * wData.size(1);
   if (overlap(out, wData) || overlap(out, wScales) || (aScales && (overlap(out, a) || overlap(out, *aScales)))) throw std::invalid_argument("out overlaps a quantised operand");
@@ -140,10 +141,22 @@ void product(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales
     check(purlin_mx4_linear(a.data_ptr(), int(type), ptr(work), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), narrow(rows), narrow(n), narrow(k), int(epilogue), nullptr, stream()));
   }
 }
+// Nothing here is differentiable. A result that was computed from a tensor with a gradient says so to whoever differentiates it; with `out`, which is
+// written in place, such a call is refused, as torch's own functions do.
+constexpr char kNoGradient[] = "a 4-bit product is not differentiable";
+void product(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales, const Tensor& wData, const Tensor& wScales, const Tensor& out, int64_t rows, int64_t epilogue) {
+  refuseTangents("a 4-bit product", {&a, &out});
+  if (at::GradMode::is_enabled() && (a.requires_grad() || out.requires_grad()))
+    throw std::runtime_error("a 4-bit product with out is not differentiable, but one of its arguments requires a gradient");
+  if (rows) multiply(a, type, aScales, wData, wScales, out, rows, epilogue);
+}
 Tensor newProduct(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales, const Tensor& wData, const Tensor& wScales, std::vector<int64_t> shape, int64_t rows,
                   int64_t epilogue) {
+  refuseTangents("a 4-bit product", {&a});
   Tensor out = at::empty(shape, wData.options().dtype(at::kBFloat16));
-  if (rows) product(a, type, aScales, wData, wScales, out, rows, epilogue);
+  if (rows) multiply(a, type, aScales, wData, wScales, out, rows, epilogue);
+  if (at::GradMode::is_enabled() && a.requires_grad())
+    torch::autograd::create_gradient_edge(out, std::make_shared<torch::autograd::Error>(kNoGradient, torch::autograd::collect_next_edges(a)));
   return out;
 }
 

@@ -2,7 +2,8 @@
 
 32 neighbouring values of a row share a power of two (a byte, e8m0); each is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it, with a sign (e2m1): 4.25
 bits a value. ``quantize_mx4`` makes such a tensor, ``mx4_gemm`` and ``mx4_gemm_swiglu`` multiply activations with a weight that was quantised once;
-both operands go to the block-scaled tensor cores as they are, sums are fp32. For inference: nothing here is differentiable.
+both operands go to the block-scaled tensor cores as they are, sums are fp32. For inference: nothing here is differentiable. A quantised tensor
+knows of no gradient; a product of a dense tensor that requires one gives a result whose differentiation raises, and is refused with ``out``.
 """
 from __future__ import annotations
 
@@ -61,7 +62,7 @@ class Mx4Tensor:
         return v.reshape(-(-rows // 128) * 128, -1)[:rows, :cols // 32].contiguous()
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The values that the tensor stands for, exact in ``dtype`` (bf16 or fp32)."""
+        """The values that the tensor stands for, exact in ``dtype`` (bf16 or fp32); they carry no gradient."""
         if dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("values come back in bf16 or fp32")
         return _native.torch_ops().mx4_dequantize(self.data, self.scales, TYPES[dtype])
@@ -88,7 +89,7 @@ def _check_dense(x: torch.Tensor) -> Tuple[int, int, int]:
 def quantize_mx4(x: torch.Tensor) -> Mx4Tensor:
     """``x [..., cols]`` (bf16, fp16 or fp32, contiguous, cols a multiple of 32) as an ``Mx4Tensor`` of its rows. A block's power of two is that of its
     largest magnitude over 4, at least 2^-127; values are rounded to the nearest of the format, ties to the even code, and above 6 times the power
-    to 6. A block that holds an infinity or a NaN stands for NaNs."""
+    to 6. A block that holds an infinity or a NaN stands for NaNs. Not differentiable: the result, and what it is dequantised to, has no gradient."""
     rows, cols, kind = _check_dense(x)
     return Mx4Tensor._of(*_native.torch_ops().mx4_quantize(x, kind, rows, cols), rows, cols)
 
@@ -115,14 +116,14 @@ def _product(a: Union[torch.Tensor, Mx4Tensor], w: Mx4Tensor, out: Optional[torc
         raise TypeError("out is a bf16 tensor")
     if out.shape != shape or out.device != w.device or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"out is a contiguous tensor of {shape} on the operands' device")
-    if rows:
-        _native.torch_ops().mx4_product(*operand, w.data, w.scales, out, rows, epilogue)
+    _native.torch_ops().mx4_product(*operand, w.data, w.scales, out, rows, epilogue)
     return out
 
 
 def mx4_gemm(a: Union[torch.Tensor, Mx4Tensor], w: Mx4Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a @ w.T`` in bf16 for ``a [..., K]``, an ``Mx4Tensor`` or a bf16, fp16 or fp32 tensor that is quantised in the call, and ``w [N, K]``; N a multiple of
-    8. One token or many. ``out`` may be (or overlap) a dense ``a``; it may not overlap a quantised operand."""
+    8. One token or many. ``out`` may be (or overlap) a dense ``a``; it may not overlap a quantised operand.
+    Not differentiable: where ``a`` requires a gradient, differentiating the result raises, and a call with ``out`` is refused."""
     return _product(a, w, out, EPI_STORE)
 
 

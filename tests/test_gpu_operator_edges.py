@@ -93,3 +93,28 @@ def test_forward_mode_derivatives_of_the_block_are_refused():
         y = gated_ffn(*leaves)
         with pytest.raises(RuntimeError, match="forward-mode"):                                      # of the backward pass
             torch.autograd.grad(y, leaves, torch.autograd.forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+def test_differentiating_a_4_bit_product_raises():
+    from purlin_b200.models.gated_mlp import GatedMLP
+    from purlin_b200.ops.mx4 import mx4_gemm, mx4_gemm_swiglu, quantize_mx4
+    w = quantize_mx4(_rand(256, 256, 1))
+    for m in (2, 300):
+        plain = _rand(m, 256, 2)
+        x = plain.clone().requires_grad_()
+        for f in (mx4_gemm, mx4_gemm_swiglu):
+            y = f(x, w)
+            assert y.requires_grad and torch.equal(y.detach(), f(plain, w))
+            with pytest.raises(RuntimeError, match="not differentiable"):
+                y.float().sum().backward()
+            with torch.no_grad():
+                assert not f(x, w).requires_grad
+            assert not f(plain, w).requires_grad and not f(quantize_mx4(x), w).requires_grad
+            out = torch.empty_like(y)
+            with pytest.raises(RuntimeError, match="not differentiable"):
+                f(x, w, out=out)
+            with torch.no_grad():
+                assert torch.equal(f(x, w, out=out), y.detach())
+        served = GatedMLP(256, 512, seed=1).quantized()
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            served(x).float().sum().backward()

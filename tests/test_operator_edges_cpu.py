@@ -93,3 +93,20 @@ def test_forward_mode_derivatives_are_refused():
                 for mode in (torch.enable_grad, torch.no_grad):
                     with mode(), pytest.raises(RuntimeError, match="forward-mode"):
                         ops.gated_ffn(*called, 0)
+
+
+def test_a_product_with_an_output_refuses_gradients_and_any_product_tangents():
+    from purlin_b200 import _native
+    ops = _native.torch_ops()
+    x, data, scales = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(64, 32, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8)
+    out = torch.zeros(4, 64, dtype=torch.bfloat16)
+    for a, o in ((x.clone().requires_grad_(), out), (x, out.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            ops.mx4_product(a, 0, None, data, scales, o, 4, 0)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.mx4_product(_dual(x), 0, None, data, scales, out, 4, 0)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.mx4_new_product(_dual(x), 0, None, data, scales, [4, 64], 4, 0)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.mx4_quantize(_dual(x), 0, 4, 64)
