@@ -149,6 +149,7 @@ void product(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales
   if (at::GradMode::is_enabled() && (a.requires_grad() || out.requires_grad()))
     throw std::runtime_error("a 4-bit product with out is not differentiable, but one of its arguments requires a gradient");
   if (rows) multiply(a, type, aScales, wData, wScales, out, rows, epilogue);
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();      // a graph that kept the old values notices
 }
 Tensor newProduct(const Tensor& a, int64_t type, const std::optional<Tensor>& aScales, const Tensor& wData, const Tensor& wScales, std::vector<int64_t> shape, int64_t rows,
                   int64_t epilogue) {

@@ -118,3 +118,18 @@ def test_differentiating_a_4_bit_product_raises():
         served = GatedMLP(256, 512, seed=1).quantized()
         with pytest.raises(RuntimeError, match="not differentiable"):
             served(x).float().sum().backward()
+
+
+def test_an_output_that_a_graph_keeps_is_noticed():
+    from purlin_b200.ops.gated_ffn import gated_ffn
+    from purlin_b200.ops.mx4 import mx4_gemm, quantize_mx4
+    h, w = _rand(16, 64, 1), quantize_mx4(_rand(64, 64, 4))
+    w_gu = _rand(64, 64, 2).requires_grad_()
+    y = gated_ffn(h, w_gu, _rand(64, 32, 3))
+    mx4_gemm(_rand(16, 64, 5), w, out=h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(torch.ones_like(y))
+    with torch.inference_mode():
+        kept = torch.empty(16, 64, dtype=torch.bfloat16, device="cuda")
+        mx4_gemm(h, w, out=kept)
+    assert torch.equal(mx4_gemm(h, w, out=kept), mx4_gemm(h, w))
