@@ -7,8 +7,12 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <cuda_runtime.h>
+
+#include <array>
 
 #include "purlin/gated_ffn.h"
 #include "purlin/mx4.h"
@@ -32,6 +36,38 @@ void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 
+// A kernel whose wait gave up leaves outputs unwritten and says so in four words, {code, where, tile, k-block}. They lie in host memory that every
+// device can write (one set each, for the life of the process, captured graphs included), so that looking at them costs a call nothing: the first
+// call on the device after such a kernel raises, whichever operator it is of, as does check_waits().
+constexpr int kMaxDevices = 64, kWordsApart = 16;
+uint32_t* waitWords(int64_t device) {
+  static uint32_t* const all = [] {
+    void* p = nullptr;
+    const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);      // (the first call may be a captured one)
+    const size_t size = size_t(kMaxDevices) * kWordsApart * sizeof(uint32_t);
+    if (cudaHostAlloc(&p, size, cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) { cudaGetLastError(); throw std::runtime_error("purlin: no host memory for the words of waits"); }
+    memset(p, 0, size);
+    return static_cast<uint32_t*>(p);
+  }();
+  if (device < 0 || device >= kMaxDevices) throw std::invalid_argument("no such device");
+  return all + device * kWordsApart;
+}
+std::array<uint32_t, 4> takeWaitReport(int64_t device) {      // and clears it
+  uint32_t* const w = waitWords(device);
+  const volatile uint32_t* v = w;
+  if (!v[0]) return {};
+  const std::array<uint32_t, 4> r{v[0], v[1], v[2], v[3]};
+  return __atomic_exchange_n(w, 0u, __ATOMIC_ACQ_REL) ? r : std::array<uint32_t, 4>{};      // (one of two threads tells)
+}
+uint32_t* status(const Tensor& on) {
+  const int64_t device = on.device().index();
+  const auto r = takeWaitReport(device);
+  if (r[0])
+    throw std::runtime_error("purlin: a wait inside an earlier kernel of the operators on cuda:" + std::to_string(device) + " gave up (where " + std::to_string(r[1]) + ", " +
+                             std::to_string(r[2]) + ", " + std::to_string(r[3]) + "): what it computed is not complete");
+  return waitWords(device);
+}
+
 // The tangent of a dual tensor (forward-mode differentiation) would be dropped without a word: the kernels see the values alone.
 void refuseTangents(const char* name, std::initializer_list<const Tensor*> inputs) {
   for (const Tensor* t : inputs)
@@ -46,7 +82,7 @@ std::tuple<Tensor, Tensor, Tensor> ffnForward(const Tensor& x, const Tensor& wGa
   if (keep) saved = bytes(int64_t(purlin_ffn_saved_bytes(narrow(tokens), narrow(intermediate))), x);
   if (tokens)
     check(purlin_ffn_forward(x.data_ptr(), wGateUp.data_ptr(), wDown.data_ptr(), h.data_ptr(), ptr(saved), y.data_ptr(), narrow(tokens), narrow(hidden), narrow(intermediate),
-                             int(activation), nullptr, stream()));
+                             int(activation), status(x), stream()));
   return {y, h, saved};
 }
 
@@ -86,7 +122,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
         Tensor work;
         if (const size_t n = purlin_ffn_workspace_bytes(narrow(tokens), narrow(hidden), narrow(intermediate), int(needs & 1), int(needs & 2), int(needs & 4))) work = bytes(int64_t(n), x);
         check(purlin_ffn_backward(x.data_ptr(), wGateUp.data_ptr(), wDown.data_ptr(), ptr(h), ptr(saved), dy.data_ptr(), ptr(dz), ptr(dx), ptr(dGateUp), ptr(dDown), ptr(work),
-                                  work.defined() ? size_t(work.numel()) : 0, narrow(tokens), narrow(hidden), narrow(intermediate), int(ctx->saved_data["activation"].toInt()), nullptr, stream()));
+                                  work.defined() ? size_t(work.numel()) : 0, narrow(tokens), narrow(hidden), narrow(intermediate), int(ctx->saved_data["activation"].toInt()), status(x), stream()));
       }
     }
     variable_list out{dx, dGateUp, dDown};
@@ -132,13 +168,13 @@ void multiply(const Tensor& a, int64_t type, const std::optional<Tensor>& aScale
   const int64_t n = wData.size(0), k = 2 * wData.size(1);
   if (overlap(out, wData) || overlap(out, wScales) || (aScales && (overlap(out, a) || overlap(out, *aScales)))) throw std::invalid_argument("out overlaps a quantised operand");
   if (aScales) {
-    check(purlin_mx4_gemm(a.data_ptr(), aScales->data_ptr(), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), narrow(rows), narrow(n), narrow(k), int(epilogue), nullptr, stream()));
+    check(purlin_mx4_gemm(a.data_ptr(), aScales->data_ptr(), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), narrow(rows), narrow(n), narrow(k), int(epilogue), status(wData), stream()));
   } else {
     Tensor work;
     size_t size = purlin_mx4_workspace_bytes(int(type), narrow(rows), narrow(k));
     if (!size && overlap(out, a)) size = size_t(rows) * size_t(k) / 2 + purlin_mx4_scale_bytes(narrow(rows), narrow(k));
     if (size) work = bytes(int64_t(size), wData);
-    check(purlin_mx4_linear(a.data_ptr(), int(type), ptr(work), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), narrow(rows), narrow(n), narrow(k), int(epilogue), nullptr, stream()));
+    check(purlin_mx4_linear(a.data_ptr(), int(type), ptr(work), wData.data_ptr(), wScales.data_ptr(), out.data_ptr(), narrow(rows), narrow(n), narrow(k), int(epilogue), status(wData), stream()));
   }
 }
 // Nothing here is differentiable. A result that was computed from a tensor with a gradient says so to whoever differentiates it; with `out`, which is
@@ -165,6 +201,8 @@ Tensor newProduct(const Tensor& a, int64_t type, const std::optional<Tensor>& aS
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   using release = py::call_guard<py::gil_scoped_release>;
+  m.def("wait_words", [](int64_t device) { return reinterpret_cast<uintptr_t>(waitWords(device)); });
+  m.def("take_wait_report", &takeWaitReport);
   m.def("gated_ffn", &gatedFfn, release());
   m.def("mx4_quantize", &quantize, release());
   m.def("mx4_dequantize", &dequantize, release());

@@ -6,7 +6,7 @@
 ``gated_ffn(x, w_gu, w_down)`` is differentiable in all three arguments; ``w_gu = interleave_gate_up(w_gate, w_up)`` is the weight
 that ``gemm_swiglu`` takes, and its gradient has the same order of rows (``split_gate_up`` gives the two parts).
 bf16 tensors, fp32 accumulation in tensor memory. Between forward and backward the block keeps ``h`` (bf16) and the pre-activations in
-24 bits, together 8 bytes per token and intermediate column.
+24 bits, together 8 bytes per token and intermediate column. Waits inside the kernels are bounded: see ``ops.waits``.
 """
 from __future__ import annotations
 

@@ -4,6 +4,7 @@
 bits a value. ``quantize_mx4`` makes such a tensor, ``mx4_gemm`` and ``mx4_gemm_swiglu`` multiply activations with a weight that was quantised once;
 both operands go to the block-scaled tensor cores as they are, sums are fp32. For inference: nothing here is differentiable. A quantised tensor
 knows of no gradient; a product of a dense tensor that requires one gives a result whose differentiation raises, and is refused with ``out``.
+Waits inside the kernels are bounded: see ``ops.waits``.
 """
 from __future__ import annotations
 

@@ -133,3 +133,57 @@ def test_an_output_that_a_graph_keeps_is_noticed():
         kept = torch.empty(16, 64, dtype=torch.bfloat16, device="cuda")
         mx4_gemm(h, w, out=kept)
     assert torch.equal(mx4_gemm(h, w, out=kept), mx4_gemm(h, w))
+
+
+def _plant(words):
+    """What a kernel whose wait gave up writes, from the host."""
+    import ctypes
+    from purlin_b200 import _native
+    at = (ctypes.c_uint32 * 4).from_address(_native.torch_ops().wait_words(torch.cuda.current_device()))
+    at[:] = words
+
+
+def test_a_wait_that_gave_up_is_told_to_the_next_call():
+    from purlin_b200.ops.gated_ffn import gated_ffn
+    from purlin_b200.ops.mx4 import mx4_gemm, quantize_mx4
+    from purlin_b200.ops.waits import check_waits
+    leaves = [v.requires_grad_() for v in (_rand(16, 64, 1), _rand(64, 64, 2), _rand(64, 32, 3))]
+    q, w = quantize_mx4(_rand(300, 64, 5)), quantize_mx4(_rand(64, 64, 4))
+    few = _rand(2, 64, 6)
+    y = gated_ffn(*leaves)
+    check_waits()
+    for call in (lambda: gated_ffn(*leaves), lambda: torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True), lambda: mx4_gemm(q, w), lambda: mx4_gemm(few, w)):
+        want = call()
+        _plant((5, 3, 17, 2))
+        with pytest.raises(RuntimeError, match="gave up.*where 3, 17, 2"):
+            call()
+        got = call()                              # told once
+        assert all(torch.equal(a, b) for a, b in zip(want, got)) if isinstance(got, tuple) else torch.equal(want, got)
+    for device in (None, 0, "cuda", "cuda:0", torch.device("cuda", 0)):
+        _plant((5, 1, 2, 3))
+        with pytest.raises(TimeoutError, match="where 1, 2, 3"):
+            check_waits(device)
+        check_waits(device)
+
+
+def test_the_words_of_waits_when_the_first_call_is_captured():
+    # a process of its own: nothing has been called before
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+from purlin_b200.ops.mx4 import mx4_gemm, quantize_mx4
+x, w = torch.ones(300, 64, device="cuda", dtype=torch.bfloat16), quantize_mx4(torch.ones(64, 64, device="cuda", dtype=torch.bfloat16))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = mx4_gemm(x, w)
+g.replay()
+assert (y == 64).all()
+from purlin_b200.ops.waits import check_waits
+check_waits()
+print("ok")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=str(Path(__file__).resolve().parent.parent))
+    assert done.returncode == 0 and done.stdout.strip().endswith("ok"), done.stdout + done.stderr
