@@ -25,11 +25,8 @@ def scale_bytes(rows: int, cols: int) -> int:
     return -(-rows // 128) * -(-cols // 128) * 512
 
 
-def _check_sizes(rows: int, cols: int):
-    if rows > MAX_ROWS:
-        raise ValueError("at most 2^30 rows")
-    if cols > MAX_COLS:
-        raise ValueError("at most 2^31 - 1056 columns")
+def _refuse_sizes(rows: int):
+    raise ValueError("at most 2^30 rows" if rows > MAX_ROWS else "at most 2^31 - 1056 columns")
 
 
 class Mx4Tensor:
@@ -43,7 +40,8 @@ class Mx4Tensor:
             raise TypeError("data and scales are uint8 tensors")
         if data.dim() != 2 or data.shape[1] == 0 or data.shape[1] % 16 or scales.numel() != scale_bytes(data.shape[0], 2 * data.shape[1]):
             raise ValueError("data is [rows, cols / 2] with cols a multiple of 32, and scales has 512 bytes for every 128 rows x 128 columns")
-        _check_sizes(data.shape[0], 2 * data.shape[1])
+        if data.shape[0] > MAX_ROWS or 2 * data.shape[1] > MAX_COLS:
+            _refuse_sizes(data.shape[0])
         if not (data.is_cuda and scales.device == data.device and data.is_contiguous() and scales.is_contiguous()):
             raise ValueError("data and scales must be contiguous CUDA tensors on one device")
         if (data.data_ptr() | scales.data_ptr()) % 16:
@@ -79,7 +77,8 @@ def _check_dense(x: torch.Tensor) -> Tuple[int, int, int]:
     if cols == 0 or cols % 32:
         raise ValueError("the last dimension must be a multiple of 32")
     rows = x.numel() // cols
-    _check_sizes(rows, cols)
+    if rows > MAX_ROWS or cols > MAX_COLS:
+        _refuse_sizes(rows)
     if not (x.is_cuda and x.is_contiguous()):
         raise ValueError("operands must be contiguous CUDA tensors")
     if x.data_ptr() % 16:
