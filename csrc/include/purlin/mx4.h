@@ -25,7 +25,7 @@ int purlin_mx4_dequantize(const void* data, const void* scales, void* out, int d
 
 /* C[M, N] = A[M, K] * W[N, K]^T, fp32 accumulation, bf16 output; A and W as above. epilogue: PURLIN_EPI_STORE or PURLIN_EPI_SWIGLU (W's rows
  * alternate 16 of gate and 16 of up, N a multiple of 32, C is [M, N / 2]). N a multiple of 8. C overlaps no operand. status: as in
- * purlin_gemm_bf16. */
+ * purlin_ffn_forward, with k-blocks of 256. */
 int purlin_mx4_gemm(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, int epilogue,
                     uint32_t* status, void* stream);
 /* The same with activations x [M, K] of `dtype`, quantised by the way: a few tokens inside the product, more into the workspace first, which has

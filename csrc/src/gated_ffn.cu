@@ -32,6 +32,7 @@
 #include "purlin/tc_sm100.cuh"
 #include "purlin/telemetry.hpp"
 #include "purlin/tensor_map.hpp"
+#include "purlin/wait_limit.hpp"
 
 using namespace purlin;
 using namespace purlin::ffn;
@@ -530,15 +531,19 @@ int launchAs(Params& p, int groups, const Shape& s, const Device& dev, cudaStrea
     }
     units = n;
   }
-  int64_t tiles = 0;
+  int64_t tiles = 0, kBlocks = 0, longest = 0;
   for (int i = 0; i < groups; ++i) {
     const Sizes z{p.g[i].t.M, p.g[i].t.N, p.g[i].t.K};
     const int tileRows = kBM * CTAS * ACCS;
     p.g[i].t.tilesM = (z.M + tileRows - 1) / tileRows; p.g[i].t.tilesN = (z.N + s.bn - 1) / s.bn;
     if (tilesOf(z, s) * p.g[i].t.split > INT32_MAX / 4) { setError("feed-forward: the product is too large"); return 1; }
     tiles += tilesOf(z, s) * p.g[i].t.split;
+    const int64_t each = (int64_t(z.K) + kBK - 1) / kBK;
+    kBlocks += tilesOf(z, s) * each;
+    longest = std::max(longest, each);
   }
   units = int(std::min<int64_t>(units, tiles));
+  p.timeoutNs = waitLimitNs(kBlocks / units + 2 * longest);
   Tiles work[kMaxGroups];
   for (int i = 0; i < groups; ++i) work[i] = p.g[i].t;
   shareOut(p.schedule, work, groups, s, units, EPI);
@@ -586,7 +591,7 @@ int run(const Product* products, int n, void* saved, void* partial, int activati
   p.bn = s.bn;
   p.partial = static_cast<float4*>(partial);
   p.saved = static_cast<uint4*>(saved); p.savedCols = EPI == kGate ? products[0].N / 32 : products[0].N / 16;
-  p.activation = activation; p.status = status; p.timeoutNs = 2ull * 1000 * 1000 * 1000;
+  p.activation = activation; p.status = status;
   auto bf16Map = [](CUtensorMap& m, const void* ptr, int rows, int cols, int boxRows) {
     return makeTensorMap(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ptr, uint64_t(rows), uint64_t(cols) * 2, uint64_t(cols) * 2, uint32_t(boxRows));
   };

@@ -22,6 +22,7 @@
 #include "purlin/tc_sm100.cuh"
 #include "purlin/telemetry.hpp"
 #include "purlin/tensor_map.hpp"
+#include "purlin/wait_limit.hpp"
 
 using namespace purlin;
 
@@ -770,7 +771,7 @@ int launchFew(const void* x, const void* aData, const void* aScales, const void*
   if (reinterpret_cast<uintptr_t>(C) % 16) { setError("TMA operands need 16-byte aligned base and row pitch"); return 1; }
   FewParams p{};
   p.N = N; p.K = K; p.tokens = M; p.cols = (M + 15) / 16 * 16;
-  p.C = static_cast<__nv_bfloat16*>(C); p.ldc = outCols; p.status = status; p.timeoutNs = 2ull * 1000 * 1000 * 1000;
+  p.C = static_cast<__nv_bfloat16*>(C); p.ldc = outCols; p.status = status; p.timeoutNs = waitLimitNs((int64_t(K) + kBK - 1) / kBK);
   const int tiles = (N + kWRows - 1) / kWRows, kBlocks = (K + kBK - 1) / kBK;
   // k is cut while that brings more CTAs to work (two to an SM) and leaves each at least four k-blocks
   int split = 1;
@@ -849,7 +850,7 @@ int launchWide(const void* aData, const void* aScales, const void* wData, const 
     pairs = n;
   }
   WideParams p{};
-  p.M = M; p.N = N; p.K = K; p.status = status; p.timeoutNs = 2ull * 1000 * 1000 * 1000;
+  p.M = M; p.N = N; p.K = K; p.status = status; p.timeoutNs = waitLimitNs(2 * ((int64_t(K) + kBK - 1) / kBK));
   p.tilesM = (M + 2 * kBM - 1) / (2 * kBM);
   // The width that is expected to take least: a tile costs its columns and about 48 columns' worth besides (fill, drain, the loads of A). Tiles of a
   // last wave that leaves pairs idle are cut where every part finds a pair (us, uncut / in halves / in quarters:

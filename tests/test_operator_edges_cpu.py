@@ -110,3 +110,12 @@ def test_a_product_with_an_output_refuses_gradients_and_any_product_tangents():
             ops.mx4_new_product(_dual(x), 0, None, data, scales, [4, 64], 4, 0)
         with pytest.raises(RuntimeError, match="forward-mode"):
             ops.mx4_quantize(_dual(x), 0, 4, 64)
+
+
+def test_no_wait_of_the_operators_has_a_fixed_limit():
+    # an epilogue waits for sums of up to 2^29 tokens, which may take longer than any limit that does not know of them
+    from pathlib import Path
+    src = Path(__file__).resolve().parent.parent / "csrc" / "src"
+    for name, launches in (("gated_ffn.cu", 1), ("mx4.cu", 2)):
+        limits = [line.split("timeoutNs =")[1] for line in (src / name).read_text().splitlines() if "timeoutNs =" in line]
+        assert len(limits) == launches and all("waitLimitNs(" in v for v in limits), name
