@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4WideKernel(const __grid_co
 // DENSE: the activations come as bf16, and the four warps that wait for the sums quantise them in the meantime, every CTA its own k range of
 // them, straight into the stages: one launch instead of two for a handful of tokens (one B200, us, two launches / one: 1 x 2048 x 2048 5.5 / 4.3, 1 x 7168 x 8192 8.9 / 7.6,
 // 4 x 57344 x 8192 43.6 / 42.0; with two tokens to a warp 50.8, so up to four tokens).
-constexpr int kFewThreads = skinny::kThreads, kWRows = 128;
+constexpr int kFewThreads = skinny::kThreads, kWRows = 128, kMostFewRows = 80;
 constexpr int kDenseTokens = 4, kDenseBytes = kDenseTokens * kBK * 2;      // a token to a warp; of bf16 activations in a stage
 
 struct FewParams {
@@ -776,8 +776,7 @@ int launchFew(const void* x, const void* aData, const void* aScales, const void*
   // k is cut while that brings more CTAs to work (two to an SM) and leaves each at least four k-blocks
   int split = 1;
   while (split < skinny::kMaxSplit && int64_t(tiles) * split * 2 <= 2 * int64_t(dev.sms) && kBlocks >= 8 * split) split *= 2;
-  const int used = (p.cols + 31) / 32 * 32 + 32;
-  p.tmemCols = used <= 64 ? 64 : used <= 128 ? 128 : 256;
+  p.tmemCols = p.cols <= 32 ? 64 : 128;      // the accumulator's columns in 32s, and 32 for scales: kMostFewRows take 96 and 32
   // the partial tile [tokens][128] in fp32 takes the place of the stages
   const int room = 113 * 1024 - 1024 - 256, stage = fewStageBytes(p.cols, x != nullptr);
   p.stages = std::max(std::min({room / stage, 8, std::max((kBlocks + split - 1) / split, 2)}), (M * kWRows * 4 + stage - 1) / stage);
@@ -820,10 +819,10 @@ bool apartFromOutput(const void* data, const void* scales, int rows, int cols, c
 // whether the product quantises its activations itself
 bool quantisedInside(int dtype, int M) { return dtype == PURLIN_MX4_BF16 && M <= kDenseTokens; }
 
-// Rows of A up to which the kernel for few rows is taken (it has room for 128). The other one does not care how many of 256 there are; us, few rows 64 /
+// Rows of A up to which the kernel for few rows is taken. The other one does not care how many of 256 there are; us, few rows 64 /
 // few rows 96 / the other: N, K 1024, 7168 6.3 / 7.3 / 9.1; 2048, 2048 5.1 / 5.6 / 5.1; 4096, 14336 13.3 / 17.1 / 15.2; 8192, 8192 few rows 64 11.3,
 // the other 10.9; 14336, 2048 7.4 and 7.5; 28672, 4096 11.2 and 14.4.
-int fewRows(int N) { return N < 8192 ? 80 : 64; }
+int fewRows(int N) { return N < 8192 ? kMostFewRows : 64; }
 
 int launchWide(const void* aData, const void* aScales, const void* wData, const void* wScales, void* C, int M, int N, int K, bool swiglu, uint32_t* status, const Device& dev,
                cudaStream_t stream) {

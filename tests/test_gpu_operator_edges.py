@@ -187,3 +187,26 @@ print("ok")
 """
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=str(Path(__file__).resolve().parent.parent))
     assert done.returncode == 0 and done.stdout.strip().endswith("ok"), done.stdout + done.stderr
+
+
+@pytest.mark.parametrize("m", [1, 31, 32, 33, 65, 66, 72, 79, 80, 81, 127, 128])
+@pytest.mark.parametrize("n,k", [(384, 2048), (1024, 28672), (8160, 4096), (8192, 4096)])
+def test_products_around_the_borders_of_the_kernel_for_few_rows(m, n, k):
+    # below 8192 columns it takes up to 80 rows, whose partial tiles and scales are the most that it holds, else up to 64; sums of whole numbers that
+    # fp32 holds exactly, so that a wrong column, row or scale cannot hide in a tolerance: the magnitudes of a block's terms add up to at most
+    # 16 * 32 + 31 * 8 * 16 = 4480, and those of 896 blocks to less than 2^24
+    from purlin_b200.ops.mx4 import mx4_gemm, quantize_mx4
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+
+    def whole(rows, most):                          # small whole numbers, a power of two to each block of 32 of a row, each block's largest is 4 times it
+        v = torch.randint(-2, 3, (rows, k), generator=g, device="cuda").float()
+        v.view(rows, -1, 32)[:, :, 0] = 4
+        power = torch.exp2(torch.randint(0, most + 1, (rows, k // 32, 1), generator=g, device="cuda").float())
+        return (v.view(rows, -1, 32) * power).view(rows, k)
+
+    a, w = whole(m, 2), whole(n, 3)
+    y = a.double() @ w.double().t()
+    assert (a.abs().double() @ w.abs().double().t()).max() < 2 ** 24
+    for x in (a, a.to(torch.bfloat16)):
+        assert torch.equal(mx4_gemm(quantize_mx4(x), quantize_mx4(w)).double(), y.to(torch.bfloat16).double())
+        assert torch.equal(mx4_gemm(x, quantize_mx4(w)).double(), y.to(torch.bfloat16).double())
