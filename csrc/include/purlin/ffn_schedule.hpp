@@ -75,7 +75,7 @@ inline int64_t tilesOf(const Sizes& z, const Shape& s) {
 }
 // Expected cycles of a tile. A k-block (64 of k) takes the longest of its MMAs (bn / 2 cycles per 16 of k and accumulator, more where they all go
 // into one), its loads from L2 (50 bytes a cycle and SM) and a round trip through the ring. The epilogue follows the main loop of a tile of two
-// accumulators and hides under the next one's with one. The constants are fitted to 326 random sizes, each tile timed on each; over 180 others the
+// accumulators and hides under the next one's with one. The constants are fitted to 326 random sizes, each tile timed on each (a sweep on one B200, no part of the tests); over 180 others the
 // choice takes 3.2 % (gate and up), 2.0 % (gate's gradient) and 2.9 % (the other gradients) longer than the best tile, where constants from
 // reasoning took 5 and 3 and 5 %. us under the power cap, 512 x 256 / 256 x 256 per pair / 128 x 256 per CTA: gradient of the gate 1000 x 3584,
 // k 8192 99 / 66 / 79; 8192 x 4096, k 1024 124 / 113 / 110; gate and up 4099 x 4096, k 7168 201 / 216 / 262; 2595 x 46560, k 424 196 / 183 / 219.

@@ -14,7 +14,7 @@ enum { PURLIN_ACT_SILU = 0, PURLIN_ACT_GELU = 1 };   /* GELU: the form with the 
 size_t purlin_ffn_saved_bytes(int tokens, int intermediate);
 
 /* hOut[tokens, I] = act(x Wg^T) * (x Wu^T), bf16, with wGateUp [2 I, hidden] (16 rows of gate and 16 of up in turn), and, where `saved` is
- * given, the pre-activations in it. y[tokens, hidden] = hOut wDown^T, unless y is NULL. All row-major, 16-byte aligned; hidden a multiple of 8,
+ * given, the pre-activations in it. y[tokens, hidden] = hOut wDown^T, unless y is NULL. No output overlaps an operand or another output, here and below. All row-major, 16-byte aligned; hidden a multiple of 8,
  * intermediate of 16. Below 2^29 of each. status: 4 words that the device can write, or NULL: {code, where, tile, k-block} of the first wait inside a
  * kernel that gave up, two seconds and 4 us for every k-block of 64 that a CTA walks; what was not finished by then is not written. */
 int purlin_ffn_forward(const void* x, const void* wGateUp, const void* wDown, void* hOut, void* saved, void* y, int tokens, int hidden,

@@ -20,7 +20,8 @@ size_t purlin_mx4_scale_bytes(int rows, int cols);
 
 /* x [rows, cols] of `dtype`, row-major, 16-byte aligned. */
 int purlin_mx4_quantize(const void* x, int dtype, void* data, void* scales, int rows, int cols, void* stream);
-/* The values that data and scales stand for, exact in bf16 or fp32 (`dtype`). */
+/* The values that data and scales stand for in bf16 or fp32 (`dtype`): exact for scale bytes up to 252, which are all that the quantisation makes (and 255);
+ * with 253 and 254 the largest of them are past both types' range and become infinities. No output overlaps an input, here and above. */
 int purlin_mx4_dequantize(const void* data, const void* scales, void* out, int dtype, int rows, int cols, void* stream);
 
 /* C[M, N] = A[M, K] * W[N, K]^T, fp32 accumulation, bf16 output; A and W as above. epilogue: PURLIN_EPI_STORE or PURLIN_EPI_SWIGLU (W's rows

@@ -61,7 +61,8 @@ class Mx4Tensor:
         return v.reshape(-(-rows // 128) * 128, -1)[:rows, :cols // 32].contiguous()
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The values that the tensor stands for, exact in ``dtype`` (bf16 or fp32); they carry no gradient."""
+        """The values that the tensor stands for in ``dtype`` (bf16 or fp32); they carry no gradient. Exact for what ``quantize_mx4`` makes; of
+        scale bytes of 253 and 254, which it never makes, the largest values are past the types' range and become infinities."""
         if dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("values come back in bf16 or fp32")
         return _native.torch_ops().mx4_dequantize(self.data, self.scales, TYPES[dtype])

@@ -210,3 +210,24 @@ def test_products_around_the_borders_of_the_kernel_for_few_rows(m, n, k):
     for x in (a, a.to(torch.bfloat16)):
         assert torch.equal(mx4_gemm(quantize_mx4(x), quantize_mx4(w)).double(), y.to(torch.bfloat16).double())
         assert torch.equal(mx4_gemm(x, quantize_mx4(w)).double(), y.to(torch.bfloat16).double())
+
+
+def test_every_code_with_every_scale_byte_that_a_caller_may_build():
+    # exact up to byte 252, NaNs at 255; between, what is past the largest number becomes an infinity
+    from purlin_b200.ops.mx4 import Mx4Tensor, scale_bytes
+    grid = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
+    codes = torch.arange(32, dtype=torch.uint8).view(1, 32).expand(256, 32) % 16
+    data = (codes[:, 0::2] | codes[:, 1::2] << 4).contiguous().cuda()
+    scales = torch.zeros(scale_bytes(256, 32), dtype=torch.uint8)
+    row = torch.arange(256)
+    scales[row // 128 * 512 + row % 32 * 16 + row // 32 % 4 * 4] = row.to(torch.uint8)
+    q = Mx4Tensor(data, scales.cuda())
+    assert torch.equal(q.scale_matrix().cpu().flatten(), row.to(torch.uint8))
+    values = torch.where(codes < 8, 1.0, -1.0).double() * grid[codes.long() % 8] * torch.pow(torch.tensor(2.0, dtype=torch.float64), row.double() - 127)[:, None]
+    values[255] = float("nan")
+    assert (values[:253].abs() < 2.0 ** 128).all()
+    for dtype in (torch.bfloat16, torch.float32):
+        got = q.dequantize(dtype).cpu()
+        want = torch.where(values.abs() >= 2.0 ** 128, values.sign() * float("inf"), values)
+        assert torch.equal(got.double().nan_to_num(nan=7.0, posinf=8.0, neginf=9.0), want.nan_to_num(nan=7.0, posinf=8.0, neginf=9.0))
+        assert got[:253].isfinite().all()
